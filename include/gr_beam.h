@@ -361,6 +361,149 @@ int32_t gr_remux_logprobs(const gr_remux_desc* desc, const int32_t* row_w, const
                           const float* lps, const void* ids, const void* ranks, const void* st,
                           float* out_lps, void* out_ids, void* out_ranks, void* out_st, void* stream);
 
+/* ---- paged KV cache of the attention pass ---------------------------------
+ *
+ * Block bookkeeping, cache write and attention over the cache for the tokens
+ * of a step: whole prompts, chunks of prompts, single decoded tokens and the
+ * beam-consecutive tokens of mega-requests, in one batch.
+ *
+ * Block tables and slot maps from request lengths, built on the device.  Row r
+ * of the block table names the cache blocks of request r in order; cached[r]
+ * tokens are there already and fresh[r] new ones join them.  With b =
+ * block_size,
+ *     have_r = ceil(cached[r] / b)      need_r = ceil((cached[r] + fresh[r]) / b)
+ *     base_r = sum over s < r of (need_s - have_s)
+ *     block_table[r][j] = free_blocks[base_r + j - have_r]     have_r <= j < need_r
+ *     cu_seqlens[r] = sum over s < r of fresh[s]   (num_seqs + 1 entries)
+ *     seq_lens[r]   = cached[r] + fresh[r]
+ *     blocks_used   = sum of (need_r - have_r)
+ * and for token t = cu_seqlens[r] + i of request r, p = cached[r] + i:
+ *     positions[t] = p      slot_mapping[t] = block_table[r][p / b] * b + p % b
+ * Token entries behind the last request's (num_tokens larger than the sum of
+ * fresh: a padded batch) get position 0 and slot -1, which gr_store_kv skips.
+ * Other entries of the block table are left as they were.
+ * A block that the free list or the table's row has no room for, or a negative
+ * id in the table, gives slot -1 and GR_DEVERR_NO_BLOCK; blocks_used still
+ * counts what the step needs.  Negative lengths, lengths whose sum leaves 32
+ * bits, and tokens beyond num_tokens give GR_DEVERR_BAD_RECORD: such a length
+ * pair counts as no new token (a negative cached as 0), such tokens have no
+ * entry.  err may be NULL; bits are OR-ed into it.  positions may be NULL.
+ * The reference leaves this to vLLM's host code (v1/worker/block_table.py,
+ * NumPy loops and copies per step); its builder consumes the result
+ * (beam_attn.py:432-476). */
+#define GR_DEVERR_NO_BLOCK      0x80  /* block tables: no free block, or no room in the row */
+
+typedef struct gr_block_table_desc {
+  int32_t num_seqs;          /* R                                                */
+  int32_t num_tokens;        /* entries of slot_mapping / positions               */
+  int32_t num_free;          /* entries of free_blocks                            */
+  int32_t block_size;        /* tokens per block, >= 1                            */
+  int32_t max_blocks;        /* entries per block table row                       */
+  int32_t reserved;
+  int64_t table_stride;      /* elements between block table rows                 */
+} gr_block_table_desc;
+
+int32_t gr_extend_block_tables(const gr_block_table_desc* desc, int32_t* block_table, const int32_t* cached,
+                               const int32_t* fresh, const int32_t* free_blocks, int32_t* cu_seqlens,
+                               int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions,
+                               int32_t* blocks_used, int32_t* err, void* stream);
+
+/* The step's new K and V rows written into the cache, the inverse of
+ * gr_suffix_kv_gather: for every token t with slot = slot_mapping[t] >= 0
+ *     k_cache[slot / block_size][slot % block_size][h][d] = k[t][h][d]
+ * and the same for V.  Slots < 0 are skipped (padding); slots outside
+ * [0, num_blocks * block_size) are skipped and set GR_DEVERR_BAD_SLOT in *err
+ * (err may be NULL).  The slots of one call must differ from one another: of two
+ * rows for one slot an unspecified mix may remain.  Strides are in elements.
+ * Replaces vLLM's reshape_and_cache_flash as the reference calls it
+ * (beam_attn.py:727-732). */
+typedef struct gr_kv_store_desc {
+  int64_t num_tokens;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t num_heads;         /* KV heads                                          */
+  int32_t head_dim;          /* elements per head                                 */
+  int32_t elem_bytes;        /* 1, 2 or 4                                         */
+  int64_t k_stride_tok, k_stride_head, k_stride_dim;                /* rows        */
+  int64_t v_stride_tok, v_stride_head, v_stride_dim;
+  int64_t kc_stride_block, kc_stride_tok, kc_stride_head, kc_stride_dim;   /* cache */
+  int64_t vc_stride_block, vc_stride_tok, vc_stride_head, vc_stride_dim;
+} gr_kv_store_desc;
+
+int32_t gr_store_kv(const gr_kv_store_desc* desc, const void* k, const void* v, void* k_cache, void* v_cache,
+                    const int64_t* slot_mapping, int32_t* err, void* stream);
+
+/* Attention of a step's query tokens over the cache.  Request r has the query
+ * tokens cu_seqlens[r] .. cu_seqlens[r+1]; n_r of them, and L_r = seq_lens[r]
+ * keys, the new tokens' own included.  Query token i sits at position p = L_r -
+ * n_r + i and sees key position k iff
+ *     causal:      k <= p              not causal:  k < L_r
+ * and, when beam_steps[r] > 0 (mega-requests, causal only), with first = L_r -
+ * n_r + beam_tail[r] the position where the beams' own tokens start:
+ *     k < first, or k >= first + floor((p - first) / steps) * steps
+ * that is, the shared prefix, the uncached prefix tail, and the own tokens of
+ * its beam.  beam_tail / beam_steps may both be NULL.  Query head h reads KV
+ * head h / (num_heads / num_kv_heads).  With s_k = scale * q.k over the seen keys
+ *     lse = ln sum_k exp(s_k)          out = sum_k exp(s_k - lse) v_k
+ * out has q's type, lse is fp32 [num_tokens][num_heads] (may be NULL).  A token
+ * that sees no key gets out = 0 and lse = -inf.  Rows of tokens that belong to
+ * no request are left as they were.
+ * Cache rows at positions >= L_r are never used, whatever they hold.  Rows at
+ * positions < L_r that a token does not see still enter as 0 * v: V has to be
+ * finite there.
+ * Replaces, for mega-requests, the reference's prefix pass, suffix gather,
+ * suffix pass and merge (beam_attn.py:629-701), and for all others its call of
+ * the paged attention kernel (beam_attn.py:734-755).
+ *
+ * Limits (GR_ERR_UNSUPPORTED): head_dim a multiple of 8 up to 256; block_size a
+ * multiple of 8; num_heads / num_kv_heads at most 128.  Strides are in elements;
+ * rows are contiguous in the head dimension, and every other stride and address
+ * of q, the caches and out must be a multiple of 16 bytes (GR_ERR_MISALIGNED).
+ * Block ids outside [0, num_blocks) read as zero rows and set
+ * GR_DEVERR_BAD_SLOT; lengths outside the table's row or the tokens set
+ * GR_DEVERR_BAD_RECORD and are clamped. */
+typedef struct gr_paged_attn_desc {
+  int32_t num_seqs;          /* R                                                */
+  int32_t num_tokens;        /* rows of q and out                                 */
+  int32_t num_heads;         /* query heads                                       */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t block_size;
+  int32_t max_blocks;        /* entries per block table row                       */
+  int32_t dtype;             /* GR_DTYPE_BF16 or GR_DTYPE_F16                     */
+  int32_t causal;            /* 0 or 1                                            */
+  int32_t max_query_len;     /* longest query of a request: picks the kernel only */
+  float scale;               /* > 0                                               */
+  int32_t reserved;
+  int64_t num_blocks;
+  int64_t table_stride;      /* elements between block table rows                 */
+  int64_t q_stride_tok, q_stride_head;
+  int64_t k_stride_block, k_stride_tok, k_stride_head;
+  int64_t v_stride_block, v_stride_tok, v_stride_head;
+  int64_t out_stride_tok, out_stride_head;
+} gr_paged_attn_desc;
+
+typedef struct gr_paged_attn_io {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* block_table;
+  const int32_t* cu_seqlens;   /* [R+1]                                           */
+  const int32_t* seq_lens;     /* [R]                                             */
+  const int32_t* beam_tail;    /* [R] or NULL                                     */
+  const int32_t* beam_steps;   /* [R] or NULL                                     */
+  void* out;
+  float* lse;                  /* [num_tokens][num_heads] or NULL                 */
+  int32_t* err;                /* device error word or NULL                       */
+} gr_paged_attn_io;
+
+/* Bytes of workspace gr_paged_attention() needs for `desc` (256-byte aligned,
+ * contents need not be initialised; calls that share it must not overlap). */
+int32_t gr_paged_attention_workspace_size(const gr_paged_attn_desc* desc, size_t* bytes);
+
+int32_t gr_paged_attention(const gr_paged_attn_desc* desc, const gr_paged_attn_io* io, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,7 +20,7 @@ STATUS_NAMES = {
 DEVERR_NAMES = {
     0x1: "GR_DEVERR_BAD_NODE", 0x2: "GR_DEVERR_BAD_CHILD", 0x4: "GR_DEVERR_TIMEOUT",
     0x8: "GR_DEVERR_OVERFLOW", 0x10: "GR_DEVERR_TIE_BOUNDARY", 0x20: "GR_DEVERR_BAD_SLOT",
-    0x40: "GR_DEVERR_BAD_RECORD",
+    0x40: "GR_DEVERR_BAD_RECORD", 0x80: "GR_DEVERR_NO_BLOCK",
 }
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 LOGPROBS_RAW, LOGPROBS_PROCESSED = 0, 1
@@ -30,6 +30,7 @@ EXPORTED_SYMBOLS = (
     "gr_abi_version", "gr_status_string", "gr_beam_step_workspace_size", "gr_beam_step",
     "gr_lse_partials", "gr_shard_candidates", "gr_merge_candidates", "gr_beam_step_noalloc",
     "gr_suffix_kv_gather", "gr_suffix_metadata", "gr_suffix_records", "gr_remux_logprobs",
+    "gr_extend_block_tables", "gr_store_kv", "gr_paged_attention_workspace_size", "gr_paged_attention",
 )
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
@@ -114,6 +115,45 @@ class KvGatherDesc(ctypes.Structure):
     ]
 
 
+class BlockTableDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_seqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_free", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+    ]
+
+
+class KvStoreDesc(ctypes.Structure):
+    _fields_ = [
+        ("num_tokens", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("elem_bytes", ctypes.c_int32),
+    ] + [(f"{t}_stride_{n}", ctypes.c_int64) for t in ("k", "v") for n in ("tok", "head", "dim")] + [
+        (f"{t}_stride_{n}", ctypes.c_int64) for t in ("kc", "vc") for n in ("block", "tok", "head", "dim")]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "num_seqs", "num_tokens", "num_heads", "num_kv_heads", "head_dim", "block_size", "max_blocks", "dtype",
+        "causal", "max_query_len")] + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)] + [
+        (n, ctypes.c_int64) for n in (
+            "num_blocks", "table_stride", "q_stride_tok", "q_stride_head", "k_stride_block", "k_stride_tok",
+            "k_stride_head", "v_stride_block", "v_stride_tok", "v_stride_head", "out_stride_tok", "out_stride_head")]
+
+
+class PagedAttnIO(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k_cache", "v_cache", "block_table", "cu_seqlens", "seq_lens", "beam_tail", "beam_steps", "out", "lse",
+        "err")]
+
+
 def describe_deverr(code: int) -> str:
     names = [n for bit, n in DEVERR_NAMES.items() if code & bit]
     return "|".join(names) if names else "0"
@@ -164,6 +204,15 @@ def load(path: str | None = None) -> ctypes.CDLL:
                                                                                 ctypes.c_void_p]
     lib.gr_remux_logprobs.restype = ctypes.c_int32
     lib.gr_remux_logprobs.argtypes = [P(RemuxDesc)] + [ctypes.c_void_p] * 11
+    lib.gr_extend_block_tables.restype = ctypes.c_int32
+    lib.gr_extend_block_tables.argtypes = [P(BlockTableDesc)] + [ctypes.c_void_p] * 11
+    lib.gr_store_kv.restype = ctypes.c_int32
+    lib.gr_store_kv.argtypes = [P(KvStoreDesc)] + [ctypes.c_void_p] * 7
+    lib.gr_paged_attention_workspace_size.restype = ctypes.c_int32
+    lib.gr_paged_attention_workspace_size.argtypes = [P(PagedAttnDesc), P(ctypes.c_size_t)]
+    lib.gr_paged_attention.restype = ctypes.c_int32
+    lib.gr_paged_attention.argtypes = [P(PagedAttnDesc), P(PagedAttnIO), ctypes.c_void_p, ctypes.c_size_t,
+                                       ctypes.c_void_p]
     _lib = lib
     return lib
 

@@ -1,0 +1,232 @@
+"""The paged KV cache of the attention pass (CUDA, sm_100a): block tables and
+slot maps from request lengths, the cache write, and attention over the blocks.
+
+A step of a batch is three calls:
+
+    m = extend_block_tables(block_table, cached, fresh, free_blocks, block_size, num_tokens)
+    store_kv(k, v, k_cache, v_cache, m["slot_mapping"])
+    out = paged_attention(q, k_cache, v_cache, block_table, m["cu_seqlens_q"], m["seq_lens"], max_seqlen_q)
+
+They take the place of what the reference's attention backend does around its
+library attention calls (vllm_gr/v1/attention/backends/beam_attn.py:629-755):
+the cache write, the paged attention of plain requests, and, for the
+beam-consecutive tokens of mega requests, prefix pass, suffix gather, suffix
+pass and merge in one call (`beam_tail` / `beam_steps`).
+
+Tensors stay on the GPU; calls run on the current stream of the tensors' device,
+do not synchronise and can be captured into CUDA graphs.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_I32, _I64 = torch.int32, torch.int64
+
+
+def _call(fn, name, device, *args):
+    """Calls an entry point on the device's current stream, with the device current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != _lib.GR_OK:
+        raise RuntimeError(f"{name} failed: {_lib.STATUS_NAMES.get(rc, rc)}")
+
+
+def _ints(name, t, device, dtype, shape=None):
+    """An index tensor as the library reads it."""
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be a {dtype} tensor on {device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _table(block_table, device, num_seqs):
+    if block_table.dtype != _I32 or block_table.device != device or block_table.dim() != 2:
+        raise ValueError(f"block_table must be a 2-D int32 tensor on {device}")
+    if block_table.shape[0] != num_seqs:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {num_seqs} requests")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table rows must have unit stride")
+    if num_seqs > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_table rows must not overlap")
+    return block_table.data_ptr()
+
+
+def _err(err, device):
+    if err is None:
+        return None
+    if err.dtype != _I32 or err.device != device:
+        raise ValueError(f"err must be an int32 tensor on {device}")
+    return err.data_ptr()
+
+
+def _cuda(t, name):
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.device
+
+
+def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_size: int, num_tokens: int, *, err=None):
+    """Grows the requests' block tables for a step's new tokens and maps the tokens to cache slots.
+
+    block_table: int32 [R, max_blocks], rows of unit stride, updated in place: request r,
+    with cached_lens[r] tokens in the cache, gets ceil((cached + new) / block_size) -
+    ceil(cached / block_size) blocks from the front of free_blocks (int32), the requests
+    in order; other entries stay as they are.  cached_lens, new_lens: int32 [R].
+    num_tokens: the step's token count, at least the sum of new_lens; entries behind that
+    sum (a padded batch) get slot -1 and position 0.
+
+    Returns a dict: cu_seqlens_q int32 [R + 1], seq_lens int32 [R] (cached + new),
+    slot_mapping int64 [num_tokens], positions int64 [num_tokens], blocks_used int32 [1]
+    (the blocks the step needs: what the caller removes from its free list).  A block that
+    the free list or a row has no room for gives slot -1 and GR_DEVERR_NO_BLOCK in `err`
+    (optional int32 device tensor), bad lengths GR_DEVERR_BAD_RECORD."""
+    device = _cuda(block_table, "block_table")
+    R, n = int(cached_lens.shape[0]) if cached_lens.dim() == 1 else -1, int(num_tokens)
+    if R < 0:
+        raise ValueError("cached_lens must be 1-D")
+    if int(block_size) < 1 or n < 0 or n > 0x7FFFFFFF or free_blocks.dim() != 1:
+        raise ValueError("block_size must be positive, num_tokens between 0 and 2^31 - 1, free_blocks 1-D")
+    d = _lib.BlockTableDesc(R, n, free_blocks.numel(), int(block_size), 0, 0, 0)
+    table = _table(block_table, device, R)
+    d.max_blocks, d.table_stride = block_table.shape[1], block_table.stride(0)
+    cached = _ints("cached_lens", cached_lens, device, _I32, (R,))
+    fresh = _ints("new_lens", new_lens, device, _I32, (R,))
+    free = _ints("free_blocks", free_blocks, device, _I32)
+    err = _err(err, device)
+    lib = _lib.load()
+    ints = torch.empty(2 * R + 2, dtype=_I32, device=device)
+    longs = torch.empty((2, n), dtype=_I64, device=device)
+    cu, lens, used = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:]
+    at = ints.data_ptr()
+    _call(lib.gr_extend_block_tables, "gr_extend_block_tables", device, d, table, cached, fresh, free, at,
+          at + 4 * (R + 1), longs.data_ptr(), longs.data_ptr() + 8 * n, at + 4 * (2 * R + 1), err)
+    return {"cu_seqlens_q": cu, "seq_lens": lens, "slot_mapping": longs[0], "positions": longs[1], "blocks_used": used}
+
+
+def _check_caches(k_cache, v_cache):
+    if k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("k_cache / v_cache must be [num_blocks, block_size, num_kv_heads, head_dim]")
+    if k_cache.dtype != v_cache.dtype or k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
+        raise ValueError("k_cache and v_cache must have the same dtype, shape and device")
+
+
+def store_kv(k, v, k_cache, v_cache, slot_mapping, *, err=None) -> None:
+    """Writes the rows k[t], v[t] ([T, num_kv_heads, head_dim]) into the cache slots
+    slot_mapping[t] (int64 [T], or int32, which is widened; slot = block * block_size +
+    offset).  Slots < 0 are skipped; slots behind the cache are skipped and set
+    GR_DEVERR_BAD_SLOT in `err`.  The slots of one call must differ.  Any strides; 1-, 2- and
+    4-byte elements; rows are copied as they are, so k and the cache have one dtype.  The
+    inverse of extract_suffix_kv."""
+    device = _cuda(k_cache, "k_cache")
+    _check_caches(k_cache, v_cache)
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != k_cache.shape[2:]:
+        raise ValueError("k and v must be [num_tokens, num_kv_heads, head_dim] with the cache's heads and head_dim")
+    if k.dtype != k_cache.dtype or v.dtype != k_cache.dtype or k.device != device or v.device != device:
+        raise ValueError("k and v must have the cache's dtype and device")
+    if k_cache.element_size() not in (1, 2, 4):
+        raise ValueError(f"unsupported KV element size {k_cache.element_size()}")
+    T = k.shape[0]
+    if slot_mapping.dtype == _I32:
+        slot_mapping = slot_mapping.to(_I64)
+    slots = _ints("slot_mapping", slot_mapping, device, _I64, (T,))
+    err = _err(err, device)
+    if T == 0 or k.shape[1] == 0 or k.shape[2] == 0:
+        return
+    nb, bs, heads, dim = k_cache.shape
+    if nb == 0 or bs == 0:
+        raise ValueError("the cache has no blocks")
+    d = _lib.KvStoreDesc(T, nb, bs, heads, dim, k_cache.element_size(), *k.stride(), *v.stride(), *k_cache.stride(),
+                         *v_cache.stride())
+    _call(_lib.load().gr_store_kv, "gr_store_kv", device, d, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
+          v_cache.data_ptr(), slots, err)
+
+
+def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seqlen_q: int, *, scale=None,
+                    causal: bool = True, beam_tail=None, beam_steps=None, out=None, return_lse: bool = False, err=None):
+    """Attention of a step's query tokens over the requests' cache blocks.
+
+    q: [T, num_heads, head_dim], bf16 or f16; caches [num_blocks, block_size, num_kv_heads,
+    head_dim] of the same dtype; block_table int32 [R, max_blocks]; cu_seqlens_q int32 [R + 1]
+    query offsets; seq_lens int32 [R] keys per request, the new tokens' own (already
+    written by store_kv) included; max_seqlen_q: the longest query, a host number that only
+    picks the kernel.  Query token i of request r sits at position seq_lens[r] - n_r + i and
+    sees the keys up to there (causal) or all of them.  Whole prompts, chunks and single
+    tokens mix freely.
+
+    beam_tail, beam_steps (int32 [R], both or neither; causal only) mark beam-consecutive
+    requests: where beam_steps[r] > 0, query tokens from beam_tail[r] on belong to beams of
+    beam_steps[r] tokens each, and a beam's tokens see the shared prefix, the tail before the
+    beams and their own beam only.
+
+    Returns out ([T, num_heads, head_dim], q's dtype; pass `out` to write into a tensor of
+    yours), with return_lse also the fp32 [T, num_heads] natural log-sum-exp of the scaled
+    scores.  A token without keys gets 0 and -inf; rows of tokens that belong to no request
+    are left as they were (unspecified in a new `out`).  scale defaults to head_dim ** -0.5.
+    V has to be finite at positions below seq_lens; what blocks hold behind does not matter.
+
+    head_dim: a multiple of 8 up to 256; block_size: a multiple of 8; num_heads /
+    num_kv_heads up to 128; unit stride in head_dim, other strides multiples of 8 elements,
+    16-byte aligned tensors.  Block ids outside the cache read as zero rows and set
+    GR_DEVERR_BAD_SLOT in `err` (optional int32 device tensor); lengths outside the table's
+    row or the tokens are clamped and set GR_DEVERR_BAD_RECORD."""
+    device = _cuda(q, "q")
+    _check_caches(k_cache, v_cache)
+    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype:
+        raise ValueError(f"q and the caches must both be bf16 or f16, not {q.dtype} and {k_cache.dtype}")
+    if q.dim() != 3 or q.shape[2] != k_cache.shape[3] or k_cache.device != device:
+        raise ValueError("q must be [num_tokens, num_heads, head_dim] with the cache's head_dim and device")
+    T, H, D = q.shape
+    nb, bs, HK, _ = k_cache.shape
+    if H == 0 or HK == 0 or D == 0 or bs == 0 or H % HK:
+        raise ValueError(f"num_heads={H} must be a multiple of num_kv_heads={HK}, sizes positive")
+    if D > 1 and (q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise ValueError("q and the caches need unit stride in head_dim")
+    if seq_lens.dim() != 1:
+        raise ValueError("seq_lens must be 1-D")
+    R = seq_lens.shape[0]
+    io = _lib.PagedAttnIO()
+    io.seq_lens = _ints("seq_lens", seq_lens, device, _I32)
+    io.cu_seqlens = _ints("cu_seqlens_q", cu_seqlens_q, device, _I32, (R + 1,))
+    io.block_table = _table(block_table, device, R)
+    if (beam_tail is None) != (beam_steps is None):
+        raise ValueError("beam_tail and beam_steps go together")
+    if beam_tail is not None:
+        if not causal:
+            raise ValueError("beams need causal attention")
+        io.beam_tail = _ints("beam_tail", beam_tail, device, _I32, (R,))
+        io.beam_steps = _ints("beam_steps", beam_steps, device, _I32, (R,))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, not {scale}")
+    if out is None:
+        out = torch.empty((T, H, D), dtype=q.dtype, device=device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or (D > 1 and out.stride(2) != 1):
+        raise ValueError("out must have q's shape, dtype and device and unit stride in head_dim")
+    lse = torch.empty((T, H), dtype=torch.float32, device=device) if return_lse else None
+    d = _lib.PagedAttnDesc(R, T, H, HK, D, bs, block_table.shape[1], _DTYPES[q.dtype], int(bool(causal)),
+                           int(max_seqlen_q), scale, 0, nb, block_table.stride(0), q.stride(0), q.stride(1),
+                           *k_cache.stride()[:3], *v_cache.stride()[:3], out.stride(0), out.stride(1))
+    lib = _lib.load()
+    size = ctypes.c_size_t(0)
+    _lib.check(lib.gr_paged_attention_workspace_size(d, size), "gr_paged_attention_workspace_size")
+    io.err = _err(err, device)
+    if T and R:
+        # from the caching allocator per call: stream ordered, and a captured graph keeps its own
+        ws = torch.empty(size.value, dtype=torch.uint8, device=device)
+        io.q, io.k_cache, io.v_cache, io.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+        io.lse = None if lse is None else lse.data_ptr()
+        _call(lib.gr_paged_attention, "gr_paged_attention", device, d, io, ws.data_ptr(), size.value)
+    return (out, lse) if return_lse else out

@@ -11,14 +11,22 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "_gr_beam.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["gr_beam_step.cu", "gr_suffix_kv.cu", "gr_remux.cu"]
-HEADERS = ["gr_device.cuh", "gr_step_ws.cuh", "gr_step_select_ws.cuh", "gr_nvtx.h"]
+OBJ_DIR = os.path.join(PKG_DIR, "build")
+# each source with the headers it includes (besides include/gr_beam.h)
+SOURCES = {
+    "gr_beam_step.cu": ["gr_device.cuh", "gr_step_ws.cuh", "gr_step_select_ws.cuh", "gr_nvtx.h"],
+    "gr_suffix_kv.cu": ["gr_nvtx.h"],
+    "gr_remux.cu": ["gr_nvtx.h"],
+    "gr_paged_kv.cu": ["gr_nvtx.h"],
+    "gr_paged_attn.cu": ["gr_device.cuh", "gr_nvtx.h"],
+}
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -33,34 +41,61 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found (set CUDA_HOME)")
 
 
-def _inputs():
-    files = [os.path.join(CSRC, s) for s in SOURCES + HEADERS]
+def _inputs(source=None):
+    files = []
+    for src, headers in SOURCES.items():
+        if source is None or src == source:
+            files += [os.path.join(CSRC, f) for f in [src, *headers]]
     files.append(os.path.join(ROOT, "include", "gr_beam.h"))
     return files
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _newer(target, files) -> bool:
+    if not os.path.exists(target):
         return False
-    t = os.path.getmtime(LIB_PATH)
-    return all(os.path.getmtime(f) <= t for f in _inputs() if os.path.exists(f))
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(f) <= t for f in files if os.path.exists(f))
 
 
-def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
-    if not force and up_to_date():
-        return LIB_PATH
-    cmd = [nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
-           "-shared", "-I", os.path.join(ROOT, "include"), "-o", LIB_PATH + ".tmp"]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += list(extra_flags or [])
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
+def up_to_date() -> bool:
+    return _newer(LIB_PATH, _inputs())
+
+
+def _run(cmd):
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stderr}")
+    return res.stderr
+
+
+def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
+    """Compiles the sources side by side (those whose object is older than what
+    it is made of; all of them with `force` or extra flags) and links them."""
+    if not force and not extra_flags and up_to_date():
+        return LIB_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    flags = [*ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include")]
     if verbose:
-        sys.stderr.write(res.stderr)
+        flags += ["-Xptxas", "-v"]
+    flags += list(extra_flags or [])
+
+    def compile_one(src):
+        obj = os.path.join(OBJ_DIR, src + ".o")
+        if not force and not extra_flags and _newer(obj, _inputs(src)):
+            return obj, ""
+        log = _run([nvcc_path(), *flags, "-c", os.path.join(CSRC, src), "-o", obj + ".tmp.o"])
+        os.replace(obj + ".tmp.o", obj)
+        return obj, log
+
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        done = list(pool.map(compile_one, SOURCES))
+    if verbose:
+        sys.stderr.write("".join(log for _, log in done))
+    _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-o", LIB_PATH + ".tmp", *[obj for obj, _ in done]])
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
+    if extra_flags:
+        for obj, _ in done:   # objects of another build than the default one are not kept
+            os.remove(obj)
     return LIB_PATH
 
 

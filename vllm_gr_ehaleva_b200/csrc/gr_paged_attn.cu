@@ -1,0 +1,1248 @@
+// gr_paged_attn.cu — attention of a step's query tokens over the paged KV cache
+// for B200 (sm_100a): whole prompts, chunks, single tokens and the beams of
+// mega-requests in one batch.
+//
+// Mathematics.  For a query row with scaled scores s_k over the keys it sees,
+// out = sum_k 2^(c s_k - m) v_k / l,  l = sum_k 2^(c s_k - m),  c = scale log2(e),
+// lse = ln2 (m + log2 l): one pass over the keys with a running reference m.  m
+// follows the running maximum only when that grows by more than 8 (a factor
+// 256), so the accumulator is rescaled rarely and no term exceeds 2^8.
+// Scores, m, l and the accumulator are fp32; the probabilities are rounded once
+// to the cache's 16-bit type as the second product's operand (each term off by
+// at most half a step, the sum l uses the unrounded ones).
+//
+// Rows.  The query heads of one KV head share its keys, so a tile of the first
+// product holds (token, head of the group) rows: tp = floor(128 / group) tokens.
+// Single tokens use group rows of the 128; their product time hides behind the
+// cache reads, which bound them.
+//
+// Work.  A unit is one key tile of one (query block, KV head); the units of the
+// whole batch, in order, are cut into equal runs, one per CTA (one persistent
+// CTA per SM), whatever the lengths.  A (block, head) cut by a run's end leaves
+// partial outputs and log-sums in the workspace, joined by a second, small
+// kernel in a fixed order.  The prefix sums of the units come from a plan: up to
+// 128 query blocks are planned by every CTA for itself, more by a one-CTA kernel
+// ahead.  For beams, key tiles between the tail and the block's first beam hold
+// only other beams' tokens and are not visited.
+//
+// Kernel.  Warp 0 loads (tensor-map copies of the blocks' rows, 128-byte
+// swizzle, a ring of key and value tiles), warp 1 issues the matrix products
+// (S = Q K^T from shared memory, O += P V with P in tensor memory), warp 2 owns
+// the tensor memory, warp 3 the plan; warps 4.. are the softmax: one thread per
+// row.  Two query tiles (kNQ = 2) have a softmax group each and alternate on the
+// tensor pipe; one tile (kNQ = 1: blocks of at most 128 rows, or heads above
+// 128) alternates two score buffers instead.
+// Every wait is bounded (GR_DEVERR_TIMEOUT).
+
+#include <cstdint>
+#include <cstdlib>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <mutex>
+
+#include "../../include/gr_beam.h"
+#include "gr_device.cuh"
+#include "gr_nvtx.h"
+
+namespace grpa {
+
+using gr::mbar_arrive;
+using gr::mbar_arrive_expect_tx;
+using gr::mbar_init;
+using gr::smem_u32;
+
+constexpr int kRows = 128;            // rows of a query tile (the matrix product's M)
+constexpr int kMaxCtas = 160;
+constexpr int kSmemPlan = 128;        // query blocks that a CTA plans for itself
+constexpr int kSmemMax = 232448;      // shared memory a CTA may have
+constexpr float kRescale = 8.0f;      // log2 of the growth of the maximum that is let stand
+
+template <int DP_, int NQ_>
+struct Shape {
+  static constexpr int DP = DP_;                       // head dim, padded to 64 / 128 / 256
+  static constexpr int NQ = NQ_;                       // query tiles per block
+  static constexpr int BN = DP == 256 ? 64 : 128;      // keys per tile
+  static constexpr int CH = DP / 64;                   // 128-byte column chunks of a row
+  static constexpr int kChunkQ = kRows * 128;          // bytes of one chunk of a query tile
+  static constexpr int kChunkKV = BN * 128;
+  static constexpr int kQTile = CH * kChunkQ;
+  static constexpr int kStage = CH * kChunkKV;
+  static constexpr int kStages = DP == 64 ? 10 : (NQ == 2 || DP == 256 ? 5 : 6);
+  static constexpr int kThreads = 128 + 128 * NQ;
+  static constexpr int kColO = 2 * BN;                 // tensor memory: S0, S1, O0, (O1)
+  static constexpr int kData = NQ * kQTile + kStages * kStage;
+  static_assert(kColO + NQ * DP <= 512, "tensor memory columns");
+};
+
+struct Shared {
+  uint64_t full[12], empty[12];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2];   // scores ready / probabilities ready
+  uint64_t pv_done[2], o_free[2];  // product into O finished / O read out
+  uint64_t drain;
+  int64_t pre[kSmemPlan + 1];
+  int32_t item[kSmemPlan];         // request | block << 8
+  int32_t num_items;
+  uint32_t tmem;
+  int abort;
+};
+
+struct Hdr {                       // a CTA's run, for the join
+  int64_t u0;                      // its first unit
+  int64_t beg, end;                // unit range of the (block, head) it starts in
+  int32_t tok0, ntok;              // that block's query tokens
+  int32_t kvh, mid;                // its KV head; whether the run starts inside it
+};
+
+struct Params {
+  const int32_t* table;
+  const int32_t* cu;
+  const int32_t* seq_lens;
+  const int32_t* tail;
+  const int32_t* steps;
+  void* out;
+  float* lse;
+  int32_t* err;
+  int64_t table_stride, num_blocks, out_tok, out_head;
+  int num_seqs, num_tokens, heads, kv_heads, group, dim;
+  int block_size, max_blocks, causal;
+  int tp;                          // query tokens per tile
+  int box;                         // rows of a block that one copy takes
+  int flags;                       // 1: copies are not issued (test hook)
+  float scale_log2, scale;
+  // plan and partials in the workspace
+  int64_t* pre;                    // [items + 1]; NULL: planned in shared memory
+  int2* item;                      // request, block
+  int32_t* num_items;
+  Hdr* hdr;
+  float* part_o;                   // [ctas][2][NQ * 128][DP]
+  float* part_lse;                 // [ctas][2][NQ * 128]
+};
+
+// ---------------------------------------------------------------- tensor core
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Everything the calling thread has issued to the tensor core so far arrives on bar when done.
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// D (tensor memory, fp32) = A (shared memory) x B (shared memory), + D when acc.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// The same with A in tensor memory.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// Shared-memory operand descriptor, 128-byte swizzle: address, the two strides
+// (all in 16-byte units), version 1, layout 2.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>((stride >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// 32 columns of this warp's 32 lanes.
+__device__ __forceinline__ void tc_ld32(uint32_t (&r)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Tensor-map copies into this CTA's shared memory (no multicast).
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+          "r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (kBf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// A wait by a whole warp.  One that gives up sets the CTA's abort flag, which
+// ends every other wait; the warp's lanes leave together or not at all.
+__device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity) {
+  const bool ok = gr::mbar_wait_bounded(bar, parity, &sh->abort);
+  if (__all_sync(0xFFFFFFFFu, ok)) return true;
+  *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+  return false;
+}
+
+// ---------------------------------------------------------------- geometry
+struct Seq {          // a request
+  int q0, n, len;     // first query token, query tokens, keys
+  int ctx;            // position of query token 0 (negative when there are fewer keys than tokens)
+  int tail, steps;    // beams (steps 0: none)
+};
+
+__device__ __forceinline__ Seq load_seq(const Params& P, int r, int* bad = nullptr) {
+  Seq s;
+  const int a = P.cu[r], b = P.cu[r + 1];
+  const int len = P.seq_lens[r];
+  const int a1 = min(max(a, 0), P.num_tokens), b1 = min(max(b, a1), P.num_tokens);
+  s.q0 = a1;
+  s.n = b1 - a1;
+  const int64_t room = static_cast<int64_t>(P.max_blocks) * P.block_size;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(len, 0)), room));
+  if (bad && (a != a1 || b != b1 || s.len != len)) *bad = 1;
+  s.ctx = s.len - s.n;
+  s.tail = s.steps = 0;
+  if (P.causal && P.steps != nullptr) {
+    s.steps = max(P.steps[r], 0);
+    s.tail = min(max(P.tail[r], 0), s.n);
+  }
+  return s;
+}
+
+// The key tiles of query tokens [t0, t1): [0, a) and [b, c) of BN keys each;
+// at least one (a block without keys still writes its rows).
+struct Tiles {
+  int a, b, n;
+};
+template <int BN>
+__device__ __forceinline__ Tiles key_tiles(const Seq& s, int causal, int t0, int t1) {
+  const int hi = causal ? min(max(s.ctx + t1, 0), s.len) : s.len;
+  const int c = (hi + BN - 1) / BN;
+  Tiles t{c, c, 0};
+  if (s.steps > 0 && t1 > s.tail) {
+    const int first = max(s.ctx + s.tail, 0);
+    const int fb = max(t0, s.tail);
+    const int own = max(s.ctx + s.tail + (fb - s.tail) / s.steps * s.steps, 0);
+    t.a = min((first + BN - 1) / BN, c);
+    t.b = min(max(own / BN, t.a), c);
+  }
+  t.n = max(t.a + c - t.b, 1);
+  return t;
+}
+
+__device__ __forceinline__ int blocks_of(const Seq& s, int per) { return (s.n + per - 1) / per; }
+
+// Inclusive sum over a warp.
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+// The plan of a small batch (at most kSmemPlan requests and query blocks, as the
+// host has bounded them), by one warp into shared memory.
+template <class S>
+__device__ void plan_warp(const Params& P, Shared* sh) {
+  const int lane = threadIdx.x & 31;
+  const int per = S::NQ * P.tp;
+  int64_t items = 0;
+  for (int r0 = 0; r0 < P.num_seqs; r0 += 32) {
+    const int r = r0 + lane;
+    int nb = 0;
+    if (r < P.num_seqs) nb = blocks_of(load_seq(P, r), per);
+    const int64_t inc = warp_scan(nb);
+    const int64_t first = items + inc - nb;
+    for (int b = 0; b < nb && first + b < kSmemPlan; ++b) sh->item[first + b] = r | (b << 8);
+    items += __shfl_sync(0xFFFFFFFFu, inc, 31);
+  }
+  if (items > kSmemPlan) items = kSmemPlan;
+  __syncwarp();
+  int64_t units = 0;
+  for (int i0 = 0; i0 < items; i0 += 32) {
+    const int i = i0 + lane;
+    int64_t u = 0;
+    if (i < items) {
+      const int r = sh->item[i] & 255, b = sh->item[i] >> 8;
+      const Seq s = load_seq(P, r);
+      u = static_cast<int64_t>(key_tiles<S::BN>(s, P.causal, b * per, min(s.n, (b + 1) * per)).n) * P.kv_heads;
+    }
+    const int64_t inc = warp_scan(u);
+    if (i < items) sh->pre[i] = units + inc - u;
+    units += __shfl_sync(0xFFFFFFFFu, inc, 31);
+  }
+  if (lane == 0) {
+    sh->pre[items] = units;
+    sh->num_items = static_cast<int>(items);
+  }
+}
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive sum over a CTA of kPlanThreads; total in `total`.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t inc = warp_scan(v);
+  __syncthreads();
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    const int64_t p = part[lane];
+    const int64_t q = warp_scan(p);
+    part[lane] = q - p;
+    if (lane == 31) part[32] = q;
+  }
+  __syncthreads();
+  total = part[32];
+  return part[warp] + inc - v;
+}
+
+// The plan of a larger batch, in the workspace: items (request, block) in order
+// and the exclusive sums of their units.
+template <int BN>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int per, int max_items) {
+  __shared__ int64_t part[33];
+  gr::pdl_trigger();
+  int64_t items = 0, total;
+  for (int r0 = 0; r0 < P.num_seqs; r0 += kPlanThreads) {
+    const int r = r0 + static_cast<int>(threadIdx.x);
+    const int nb = r < P.num_seqs ? blocks_of(load_seq(P, r), per) : 0;
+    const int64_t first = items + block_scan(nb, total, part);
+    for (int b = 0; b < nb && first + b < max_items; ++b) P.item[first + b] = make_int2(r, b);
+    items += total;
+  }
+  if (items > max_items) items = max_items;
+  __syncthreads();
+  int64_t units = 0;
+  for (int64_t i0 = 0; i0 < items; i0 += kPlanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int64_t u = 0;
+    if (i < items) {
+      const int2 it = P.item[i];
+      const Seq s = load_seq(P, it.x);
+      u = static_cast<int64_t>(key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n) * P.kv_heads;
+    }
+    const int64_t ex = block_scan(u, total, part);
+    if (i < items) P.pre[i] = units + ex;
+    units += total;
+  }
+  if (threadIdx.x == 0) {
+    P.pre[items] = units;
+    P.num_items[0] = static_cast<int>(items);
+  }
+}
+
+// A CTA's run of units and the (block, head) pairs in it, walked alike by every role.
+struct Walk {
+  const int64_t* pre;
+  int items, i;
+  int64_t u, end;
+};
+
+struct Work {
+  Seq s;
+  int t0, nt;        // query tokens of the block, from t0 of the request
+  int kvh;
+  Tiles tiles;
+  int j0, j1;        // key tiles of the run
+  int slots;         // query tiles with rows
+  int64_t beg;       // unit range of the (block, head)
+};
+
+template <class S>
+__device__ __forceinline__ Walk walk_begin(const Params& P, const Shared* sh, int cta, int ctas) {
+  Walk w;
+  w.pre = P.pre ? P.pre : sh->pre;
+  w.items = P.pre ? P.num_items[0] : sh->num_items;
+  const int64_t units = w.pre[w.items];
+  w.u = units * cta / ctas;
+  w.end = units * (cta + 1) / ctas;
+  int lo = 0, hi = w.items > 0 ? w.items - 1 : 0;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (w.pre[mid] <= w.u) lo = mid; else hi = mid - 1;
+  }
+  w.i = lo;
+  return w;
+}
+
+template <class S>
+__device__ __forceinline__ bool walk_next(const Params& P, const Shared* sh, Walk& w, Work& k) {
+  if (w.u >= w.end) return false;
+  while (w.pre[w.i + 1] <= w.u) ++w.i;
+  int r, b;
+  if (P.pre) {
+    const int2 it = P.item[w.i];
+    r = it.x;
+    b = it.y;
+  } else {
+    r = sh->item[w.i] & 255;
+    b = sh->item[w.i] >> 8;
+  }
+  const int per = S::NQ * P.tp;
+  k.s = load_seq(P, r);
+  k.t0 = b * per;
+  k.nt = min(k.s.n - k.t0, per);
+  k.tiles = key_tiles<S::BN>(k.s, P.causal, k.t0, k.t0 + k.nt);
+  const int64_t in = w.u - w.pre[w.i];
+  k.kvh = static_cast<int>(in / k.tiles.n);
+  k.j0 = static_cast<int>(in - static_cast<int64_t>(k.kvh) * k.tiles.n);
+  k.j1 = static_cast<int>(min(static_cast<int64_t>(k.tiles.n), k.j0 + (w.end - w.u)));
+  k.slots = k.nt > P.tp ? 2 : 1;
+  k.beg = w.u - k.j0;
+  w.u += k.j1 - k.j0;
+  return true;
+}
+
+__device__ __forceinline__ int tile_at(const Tiles& t, int j) { return j < t.a ? j : j - t.a + t.b; }
+
+// ---------------------------------------------------------------- roles
+template <class S>
+struct Ring {        // position in the ring of key and value tiles
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == S::kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Warp 0: the block's queries once, then its key and value tiles in the order
+// in which the matrix products first use them.
+template <class S>
+__device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t data, const CUtensorMap* mq,
+                                          const CUtensorMap* mk, const CUtensorMap* mv, int ctas) {
+  const int lane = threadIdx.x & 31;
+  Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
+  Work k;
+  Ring<S> ring;
+  uint32_t qphase = 0;
+  int64_t issued = 0;
+  bool q_issued = false, ok = true;
+  const uint32_t ringbase = data + S::NQ * S::kQTile;
+  const int boxes = S::BN / P.box;
+  const int oob = static_cast<int>(P.num_blocks);
+  int bad = 0;
+  while (ok && walk_next<S>(P, sh, w, k)) {
+    if (!wait(sh, &sh->q_empty, qphase ^ 1u)) { ok = false; break; }
+    if (lane == 0) {
+      const int slots = S::NQ == 2 ? k.slots : 1;
+      const uint32_t bytes = static_cast<uint32_t>(slots * S::CH * P.group * P.tp * 128);
+      if (!(P.flags & 1)) {
+        mbar_arrive_expect_tx(&sh->q_full, bytes);
+        for (int q = 0; q < slots; ++q)
+          for (int c = 0; c < S::CH; ++c)
+            tma_load3(data + q * S::kQTile + c * S::kChunkQ, mq, c * 64, k.kvh * P.group, k.s.q0 + k.t0 + q * P.tp,
+                      &sh->q_full);
+        q_issued = true;
+      }
+    }
+    qphase ^= 1u;
+    const int n = k.j1 - k.j0;
+    const int lead = S::NQ == 2 ? 1 : 2;
+    const int req_row = P.pre ? P.item[w.i].x : (sh->item[w.i] & 255);
+    const int32_t* row = P.table + req_row * P.table_stride;
+    // the order K0 .. K(lead-1), V0, K(lead), V1, ...
+    for (int x = 0, ki = 0, vi = 0; x < 2 * n; ++x) {
+      const bool is_k = ki < n && ki < vi + lead;
+      const int j = is_k ? ki++ : vi++;
+      const int key0 = tile_at(k.tiles, k.j0 + j) * S::BN;
+      // this lane's boxes: the block ids first, so that their latency overlaps the wait
+      int id[2] = {oob, oob};   // box at lane, at lane + 32 (BN / 8 * CH <= 64)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int bx = (lane + 32 * h) / S::CH;
+        const int tok = key0 + bx * P.box;
+        if (bx < boxes && tok < k.s.len) {
+          const int v = __ldg(row + tok / P.block_size);
+          if (v < 0 || v >= oob) bad = 1; else id[h] = v;
+        }
+      }
+      if (!wait(sh, &sh->empty[ring.stage], ring.phase ^ 1u)) { ok = false; break; }
+      if (!(P.flags & 1)) {
+        if (lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
+        __syncwarp();
+        const uint32_t dst = ringbase + ring.stage * S::kStage;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int e = lane + 32 * h, bx = e / S::CH, c = e % S::CH;
+          if (bx < boxes) {
+            const int tok = key0 + bx * P.box;
+            tma_load4(dst + c * S::kChunkKV + bx * P.box * 128, is_k ? mk : mv, c * 64, k.kvh, tok % P.block_size, id[h],
+                      &sh->full[ring.stage]);
+          }
+        }
+        ++issued;
+      }
+      ring.next();
+    }
+  }
+  if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_SLOT);
+  if (!ok) {
+    // gave up: wait (bounded) for the copies in flight before the shared memory goes
+    int64_t left = issued < S::kStages ? issued : S::kStages;
+    for (; left > 0; --left) {
+      if (ring.stage == 0) {
+        ring.stage = S::kStages;
+        ring.phase ^= 1u;
+      }
+      --ring.stage;
+      gr::mbar_wait_bounded(&sh->full[ring.stage], ring.phase);
+    }
+    if (__any_sync(0xFFFFFFFFu, q_issued)) gr::mbar_wait_bounded(&sh->q_full, qphase ^ 1u);
+  }
+}
+
+// Value rows behind the last key hold whatever the block held before, and
+// 0 * NaN is NaN: they are zeroed before the product reads them.
+template <class S>
+__device__ __forceinline__ void zero_tail(uint32_t tile, int from, int to) {
+  const int lane = threadIdx.x & 31;
+  for (int e = lane; e < (to - from) * 8 * S::CH; e += 32) {
+    const int c = e / ((to - from) * 8), x = e - c * (to - from) * 8;
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * S::kChunkKV + from * 128 + x * 16), "r"(0)
+                 : "memory");
+  }
+  gr::fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Warp 1: the matrix products, issued by one lane.
+template <class S, bool kBf16>
+__device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t data, int ctas) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t tmem = sh->tmem;
+  const uint32_t ringbase = data + S::NQ * S::kQTile;
+  constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
+  // fp32 accumulators, A and B of one type, M = 128; B of the second product is stored along N
+  constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((S::BN / 8) << 17) | ((kRows / 16) << 24);
+  constexpr uint32_t kIdescO =
+      (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((S::DP / 8) << 17) | ((kRows / 16) << 24);
+
+  const auto qk = [&](int q, int buf, int stage) {   // S[buf] = Q[q] K^T
+    if (lane == 0) {
+      const uint32_t qa = data + q * S::kQTile, ka = ringbase + stage * S::kStage;
+#pragma unroll
+      for (int c = 0; c < S::CH; ++c)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          tc_mma_ss(tmem + buf * S::BN, smem_desc(qa + c * S::kChunkQ + x * 32, 16, 1024),
+                    smem_desc(ka + c * S::kChunkKV + x * 32, 16, 1024), kIdescS, (c | x) != 0);
+      tc_commit(&sh->s_full[buf]);
+    }
+    __syncwarp();
+  };
+  const auto pv = [&](int q, int buf, int stage, bool first) {   // O[q] (+)= P[buf] V
+    if (lane == 0) {
+      const uint32_t va = ringbase + stage * S::kStage;
+#pragma unroll
+      for (int x = 0; x < S::BN / 16; ++x)
+        tc_mma_ts(tmem + S::kColO + q * S::DP, tmem + buf * S::BN + x * 8,
+                  smem_desc(va + x * 2048, S::kChunkKV, 1024), kIdescO, !(first && x == 0));
+      tc_commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
+    }
+    __syncwarp();
+  };
+  const auto commit = [&](uint64_t* bar) {
+    if (lane == 0) tc_commit(bar);
+    __syncwarp();
+  };
+
+  Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
+  Work k;
+  Ring<S> ring;
+  uint32_t qphase = 0, pphase = 0, ofree = 3;   // one bit per buffer / tile
+  uint32_t step = 0;    // score buffer of the next step (kNQ = 1)
+  while (walk_next<S>(P, sh, w, k)) {
+    const int n = k.j1 - k.j0;
+    if (!wait(sh, &sh->q_full, qphase)) return;
+    qphase ^= 1u;
+    int kstage = 0;
+    const auto take = [&](int& stage) {
+      if (!wait(sh, &sh->full[ring.stage], ring.phase)) return false;
+      tc_fence_after();
+      stage = ring.stage;
+      ring.next();
+      return true;
+    };
+    const auto take_v = [&](int& stage, int j) {
+      if (!take(stage)) return false;
+      const int key0 = tile_at(k.tiles, k.j0 + j) * S::BN;
+      const int live = k.s.len - key0;
+      if (live > 0 && live < S::BN && live % P.box != 0)
+        zero_tail<S>(ringbase + stage * S::kStage, live, (live / P.box + 1) * P.box);
+      return true;
+    };
+    if (S::NQ == 2) {
+      if (!take(kstage)) return;
+      for (int q = 0; q < k.slots; ++q) qk(q, q, kstage);
+      commit(&sh->empty[kstage]);
+      if (n == 1) commit(&sh->q_empty);
+      for (int j = 0; j < n; ++j) {
+        int vstage = 0;
+        for (int q = 0; q < k.slots; ++q) {
+          if (!wait(sh, &sh->p_full[q], (pphase >> q) & 1u)) return;
+          pphase ^= 1u << q;
+          if (q == 0 && !take_v(vstage, j)) return;
+          if (j == 0) {
+            if (!wait(sh, &sh->o_free[q], (ofree >> q) & 1u)) return;
+            ofree ^= 1u << q;
+          }
+          tc_fence_after();
+          pv(q, q, vstage, j == 0);
+          if (q == k.slots - 1) commit(&sh->empty[vstage]);
+          if (j + 1 < n) {
+            if (q == 0 && !take(kstage)) return;
+            qk(q, q, kstage);
+            if (q == k.slots - 1) {
+              commit(&sh->empty[kstage]);
+              if (j + 2 == n) commit(&sh->q_empty);
+            }
+          }
+        }
+      }
+    } else {
+      for (int j = 0; j < 2 && j < n; ++j) {
+        if (!take(kstage)) return;
+        qk(0, (step + j) & 1, kstage);
+        commit(&sh->empty[kstage]);
+        if (j + 1 == n) commit(&sh->q_empty);
+      }
+      for (int j = 0; j < n; ++j, ++step) {
+        const int b = step & 1;
+        int vstage = 0;
+        if (!wait(sh, &sh->p_full[b], (pphase >> b) & 1u)) return;
+        pphase ^= 1u << b;
+        if (!take_v(vstage, j)) return;
+        if (j == 0) {
+          if (!wait(sh, &sh->o_free[0], ofree & 1u)) return;
+          ofree ^= 1u;
+        }
+        tc_fence_after();
+        pv(0, b, vstage, j == 0);
+        commit(&sh->empty[vstage]);
+        if (j + 2 < n) {
+          if (!take(kstage)) return;
+          qk(0, b, kstage);
+          commit(&sh->empty[kstage]);
+          if (j + 3 == n) commit(&sh->q_empty);
+        }
+      }
+    }
+  }
+}
+
+// Warps 4..: softmax of one query tile, one thread per row; also the rare
+// rescaling of the accumulator, and the block's output.
+template <class S, bool kBf16>
+__device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int slot, int ctas) {
+  constexpr int BN = S::BN, DP = S::DP;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
+  const int m_row = warp * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+  const uint32_t tmem = sh->tmem + lanes;
+  const uint32_t o_col = tmem + S::kColO + slot * DP;
+  const float c = P.scale_log2;
+  const int ti = m_row / P.group, g = m_row - ti * P.group;
+  Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
+  Work k;
+  uint32_t sphase = 0, pvphase = 0;   // one bit per buffer
+  uint32_t step = 0;
+  while (walk_next<S>(P, sh, w, k)) {
+    if (S::NQ == 2 && slot >= k.slots) continue;
+    const int n = k.j1 - k.j0;
+    // this row: token, position, the keys it sees
+    const int tok = k.t0 + slot * P.tp + ti;              // in the request
+    const bool live = ti < P.tp && ti + slot * P.tp < k.nt;
+    const int pos = k.s.ctx + tok;
+    int lim = P.causal ? min(pos + 1, k.s.len) : k.s.len;
+    int first = 0x7FFFFFFF, own = 0;
+    if (k.s.steps > 0 && tok >= k.s.tail) {
+      first = k.s.ctx + k.s.tail;
+      own = first + (tok - k.s.tail) / k.s.steps * k.s.steps;
+    }
+    if (!live) lim = 0x7FFFFFFF, first = 0x7FFFFFFF;      // rows of no token: no mask, nothing stored
+    const bool any_live = __any_sync(0xFFFFFFFFu, live);
+    float m = -kInf, l = 0.0f;
+    for (int j = 0; j < n; ++j) {
+      const int b = S::NQ == 2 ? slot : static_cast<int>((step + j) & 1);
+      const int key0 = tile_at(k.tiles, k.j0 + j) * BN;
+      if (!wait(sh, &sh->s_full[b], (sphase >> b) & 1u)) return;
+      sphase ^= 1u << b;
+      tc_fence_after();
+      // which product into O has finished when: kNQ = 2 orders it before these
+      // scores, kNQ = 1 does not (the other buffer's is still to come)
+      if (any_live) {
+        const uint32_t s_col = tmem + b * BN;
+        uint32_t sr[BN / 32][32];
+#pragma unroll
+        for (int x = 0; x < BN / 32; ++x) tc_ld32(sr[x], s_col + x * 32);
+        tc_wait_ld();
+        const bool whole = key0 + BN <= lim && (key0 + BN <= first || key0 >= own);
+        if (!__all_sync(0xFFFFFFFFu, whole)) {
+          const int nl = lim - key0, nf = first - key0, no = own - key0;
+#pragma unroll
+          for (int x = 0; x < BN; ++x) {
+            const bool see = x < nl && (x < nf || x >= no);
+            if (!see) sr[x / 32][x % 32] = 0xFF800000u;
+          }
+        }
+        float t0 = -kInf, t1 = -kInf, t2 = -kInf, t3 = -kInf;
+#pragma unroll
+        for (int x = 0; x < BN; x += 4) {
+          t0 = fmaxf(t0, __uint_as_float(sr[x / 32][x % 32]));
+          t1 = fmaxf(t1, __uint_as_float(sr[x / 32][x % 32 + 1]));
+          t2 = fmaxf(t2, __uint_as_float(sr[x / 32][x % 32 + 2]));
+          t3 = fmaxf(t3, __uint_as_float(sr[x / 32][x % 32 + 3]));
+        }
+        const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+        // a reference of its own for the row's first keys, then only when the growth is large
+        const bool grow = live && ((top - m) * c > kRescale || (m == -kInf && top > -kInf));
+        if (__any_sync(0xFFFFFFFFu, grow)) {
+          const float f = grow ? gr::fast_exp2((m - top) * c) : 1.0f;   // m = -inf: 0
+          if (grow) m = top;
+          if (j > 0) {
+            if (S::NQ == 1) {
+              const int pb = b ^ 1;   // the previous key tile's product
+              if (!wait(sh, &sh->pv_done[pb], ((pvphase >> pb) & 1u) ^ 1u)) return;
+              tc_fence_after();
+            }
+            l *= f;
+#pragma unroll 1
+            for (int x = 0; x < DP; x += 32) {
+              uint32_t o[32];
+              tc_ld32(o, o_col + x);
+              tc_wait_ld();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+              tc_st32(o_col + x, o);
+            }
+            tc_wait_st();
+          }
+        }
+        const float mc = m == -kInf ? 0.0f : m * c;
+        const uint64_t c2 = gr::pack2(c, c), n2 = gr::pack2(-mc, -mc);
+        uint64_t a0 = 0, a1 = 0;   // (0.0f, 0.0f)
+#pragma unroll
+        for (int h = 0; h < BN / 64; ++h) {
+          uint32_t p[32];
+#pragma unroll
+          for (int x = 0; x < 64; x += 2) {
+            const int y = h * 64 + x;
+            const uint64_t t = gr::ffma2(
+                gr::pack2(__uint_as_float(sr[y / 32][y % 32]), __uint_as_float(sr[y / 32][y % 32 + 1])), c2, n2);
+            float e0, e1;
+            gr::unpack2(t, e0, e1);
+            e0 = gr::fast_exp2(e0);
+            e1 = gr::fast_exp2(e1);
+            if (x & 2) a1 = gr::fadd2(a1, gr::pack2(e0, e1)); else a0 = gr::fadd2(a0, gr::pack2(e0, e1));
+            p[x / 2] = pack16<kBf16>(e0, e1);
+          }
+          tc_st32(s_col + h * 32, p);
+        }
+        tc_wait_st();
+        a0 = gr::fadd2(a0, a1);
+        float x0, x1;
+        gr::unpack2(a0, x0, x1);
+        l += x0 + x1;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->p_full[b]);
+      pvphase ^= 1u << b;   // the parity of this tile's product, once flipped back
+    }
+    // the last product into O
+    const int lb = S::NQ == 2 ? slot : static_cast<int>((step + n - 1) & 1);
+    if (!wait(sh, &sh->pv_done[lb], ((pvphase >> lb) & 1u) ^ 1u)) return;
+    tc_fence_after();
+    if (S::NQ == 1) step += n;
+    const bool whole = k.j0 == 0 && k.j1 == k.tiles.n;
+    if (any_live) {
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const float lse2 = l > 0.0f || l != l ? m * c + __log2f(l) : -kInf;
+      const int64_t t = static_cast<int64_t>(k.s.q0) + tok;
+      const int h = k.kvh * P.group + g;
+      const int part = blockIdx.x * 2 + (k.j0 == 0 ? 1 : 0);
+      const int prow = slot * kRows + m_row;
+      if (live) {
+        if (whole) {
+          if (P.lse) P.lse[t * P.heads + h] = lse2 * 0.6931471805599453f;
+        } else {
+          P.part_lse[static_cast<int64_t>(part) * S::NQ * kRows + prow] = lse2;
+        }
+      }
+      unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
+      float* prt = P.part_o + (static_cast<int64_t>(part) * S::NQ * kRows + prow) * DP;
+#pragma unroll 1
+      for (int x = 0; x < DP; x += 32) {
+        uint32_t o[32];
+        tc_ld32(o, o_col + x);
+        tc_wait_ld();
+        if (live) {
+          if (whole) {
+#pragma unroll
+            for (int y = 0; y < 32; y += 8) {
+              if (x + y < P.dim) {
+                uint4 v;
+                v.x = pack16<kBf16>(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv);
+                v.y = pack16<kBf16>(__uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
+                v.z = pack16<kBf16>(__uint_as_float(o[y + 4]) * inv, __uint_as_float(o[y + 5]) * inv);
+                v.w = pack16<kBf16>(__uint_as_float(o[y + 6]) * inv, __uint_as_float(o[y + 7]) * inv);
+                *reinterpret_cast<uint4*>(orow + (x + y) * 2) = v;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int y = 0; y < 32; y += 4)
+              *reinterpret_cast<float4*>(prt + x + y) =
+                  make_float4(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv,
+                              __uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
+          }
+        }
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->o_free[slot]);
+  }
+}
+
+template <class S, bool kBf16>
+__global__ void __launch_bounds__(S::kThreads, 1)
+    attention_kernel(const Params P, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                     const __grid_constant__ CUtensorMap mv) {
+  extern __shared__ unsigned char raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  Shared* sh = reinterpret_cast<Shared*>(raw + (base - smem_u32(raw)) + S::kData);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->empty[i], 1);
+    }
+    mbar_init(&sh->q_full, 1);
+    mbar_init(&sh->q_empty, 1);
+    mbar_init(&sh->drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh->s_full[i], 1);
+      mbar_init(&sh->p_full[i], 4);
+      mbar_init(&sh->pv_done[i], 1);
+      mbar_init(&sh->o_free[i], 4);
+    }
+    sh->abort = 0;
+    gr::fence_mbar_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  gr::pdl_wait();      // the plan (or whatever came before) is complete
+  gr::pdl_trigger();
+  if (warp == 3 && P.pre == nullptr) plan_warp<S>(P, sh);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  // units per CTA: as many CTAs as there are units to share, at most the grid
+  const int64_t units = P.pre ? P.pre[P.num_items[0]] : sh->pre[sh->num_items];
+  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), units));
+  const bool busy = static_cast<int>(blockIdx.x) < ctas;
+  if (warp == 3) {
+    // the run's header for the join, and the requests' lengths checked once
+    if (lane == 0) {
+      Hdr h{units, 0, 0, 0, 0, 0, 0};
+      if (busy) {
+        Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
+        Work k;
+        h.u0 = w.u;
+        if (walk_next<S>(P, sh, w, k)) {
+          h.beg = k.beg;
+          h.end = k.beg + k.tiles.n;
+          h.tok0 = k.s.q0 + k.t0;
+          h.ntok = k.nt;
+          h.kvh = k.kvh;
+          h.mid = k.j0 > 0;
+        }
+      }
+      P.hdr[blockIdx.x] = h;
+    }
+    int bad = 0;
+    for (int r = blockIdx.x * 32 + lane; r < P.num_seqs; r += gridDim.x * 32) load_seq(P, r, &bad);
+    if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_RECORD);
+  }
+  // registers of the two-tile kernel: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168, what the launch has
+  if (warp < 4) {
+    if constexpr (S::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 && busy) {
+      load_role<S>(P, sh, base, &mq, &mk, &mv, ctas);
+    } else if (warp == 1 && busy) {
+      mma_role<S, kBf16>(P, sh, base, ctas);
+      if (sh->abort) {   // products in flight finish before the tensor memory goes
+        if (lane == 0) tc_commit(&sh->drain);
+        __syncwarp();
+        gr::mbar_wait_bounded(&sh->drain, 0);
+      }
+    }
+  } else {
+    if constexpr (S::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if (busy) softmax_role<S, kBf16>(P, sh, (warp >> 2) - 1, ctas);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0 && sh->abort && P.err) atomicOr(P.err, GR_DEVERR_TIMEOUT);
+  if (warp == 2) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem));
+  }
+}
+
+// ---------------------------------------------------------------- join
+// One CTA row of the grid per run boundary: the first boundary inside a (block,
+// head) joins all its parts, in run order, with weights 2^(lse_i - max).
+constexpr int kJoinThreads = 128;
+constexpr int kJoinSlices = 4;
+
+template <int DP, int NQ, bool kBf16>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int ctas) {
+  gr::pdl_wait();
+  const int c = blockIdx.x + 1;
+  const Hdr h = P.hdr[c];
+  if (!h.mid || P.hdr[c - 1].u0 > h.beg) return;
+  int last = c;                              // the last run with a part of it
+  while (last + 1 < ctas && P.hdr[last + 1].u0 < h.end) ++last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = h.ntok * P.group;
+  for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows; r += kJoinSlices * (kJoinThreads / 32)) {
+    const int tok = r / P.group, g = r - tok * P.group;
+    const int slot = tok / P.tp;
+    const int prow = slot * kRows + (tok - slot * P.tp) * P.group + g;
+    const auto at = [&](int i) { return static_cast<int64_t>(i * 2 + (i == c - 1 ? 1 : 0)) * NQ * kRows + prow; };
+    float top = -kInf;
+    for (int i = c - 1 + lane; i <= last; i += 32) top = fmaxf(top, P.part_lse[at(i)]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float ref = top == -kInf ? 0.0f : top;
+    float acc[DP / 32];
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) acc[x] = 0.0f;
+    float sum = 0.0f;
+    for (int i = c - 1; i <= last; ++i) {
+      const float wgt = gr::fast_exp2(P.part_lse[at(i)] - ref);
+      const float* o = P.part_o + at(i) * DP;
+      sum += wgt;
+#pragma unroll
+      for (int x = 0; x < DP / 64; ++x) {
+        const float2 v = *reinterpret_cast<const float2*>(o + x * 64 + lane * 2);
+        acc[2 * x] += wgt * v.x;
+        acc[2 * x + 1] += wgt * v.y;
+      }
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const int64_t t = static_cast<int64_t>(h.tok0) + tok;
+    const int head = h.kvh * P.group + g;
+    unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + head * P.out_head) * 2;
+#pragma unroll
+    for (int x = 0; x < DP / 64; ++x) {
+      const int col = x * 64 + lane * 2;
+      if (col < P.dim)
+        *reinterpret_cast<uint32_t*>(orow + col * 2) = pack16<kBf16>(acc[2 * x] * inv, acc[2 * x + 1] * inv);
+    }
+    if (lane == 0 && P.lse)
+      P.lse[t * P.heads + head] =
+          sum > 0.0f || sum != sum ? (ref + __log2f(sum)) * 0.6931471805599453f : -kInf;
+  }
+}
+
+// ---------------------------------------------------------------- host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static std::mutex g_mu;
+static int g_sms[64];
+static bool g_attr[64][6][2];
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+struct Geometry {
+  int dp, nq, bn, group, tp, box;
+  int64_t max_items;
+};
+
+// What the descriptor allows, and the kernel that it picks.
+static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
+  if (!d) return GR_ERR_NULL;
+  if (d->num_seqs < 0 || d->num_tokens < 0 || d->num_heads <= 0 || d->num_kv_heads <= 0 || d->head_dim <= 0 ||
+      d->block_size <= 0 || d->max_blocks < 0 || d->num_blocks < 0 || d->num_blocks >= 0x7FFFFFFF ||
+      d->num_heads % d->num_kv_heads != 0 || (d->causal != 0 && d->causal != 1) || d->max_query_len < 0 ||
+      !(d->scale > 0.0f) || d->scale > 3.0e38f || (d->num_seqs > 1 && d->table_stride < d->max_blocks) ||
+      static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7FFFFFFF - 256)
+    return GR_ERR_BAD_DESC;
+  if (d->dtype != GR_DTYPE_BF16 && d->dtype != GR_DTYPE_F16) return GR_ERR_DTYPE;
+  g.group = d->num_heads / d->num_kv_heads;
+  if (d->head_dim % 8 != 0 || d->head_dim > 256 || d->block_size % 8 != 0 || g.group > kRows) return GR_ERR_UNSUPPORTED;
+  g.dp = d->head_dim <= 64 ? 64 : (d->head_dim <= 128 ? 128 : 256);
+  g.tp = kRows / g.group;
+  // one query tile where the longest query fits it, or the accumulators of two do not
+  g.nq = (g.dp == 256 || static_cast<int64_t>(d->max_query_len) <= g.tp) ? 1 : 2;
+  g.bn = g.dp == 256 ? 64 : 128;
+  g.box = 8;
+  while (g.box * 2 <= g.bn && d->block_size % (g.box * 2) == 0) g.box *= 2;
+  const int64_t per = static_cast<int64_t>(g.nq) * g.tp;
+  g.max_items = static_cast<int64_t>(d->num_tokens) / per + d->num_seqs;
+  if (g.max_items > 0x7FFFFFFF) return GR_ERR_UNSUPPORTED;
+  return GR_OK;
+}
+
+static bool plan_in_cta(const gr_paged_attn_desc* d, const Geometry& g) {
+  return d->num_seqs <= kSmemPlan && g.max_items <= kSmemPlan;
+}
+
+static size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+struct Layout {
+  size_t hdr, part_lse, part_o, pre, item, count, total;
+};
+static Layout layout(const gr_paged_attn_desc* d, const Geometry& g) {
+  Layout l{};
+  size_t at = 0;
+  const auto take = [&](size_t n) {
+    const size_t here = at;
+    at += round256(n);
+    return here;
+  };
+  l.hdr = take(sizeof(Hdr) * kMaxCtas);
+  l.part_lse = take(sizeof(float) * kMaxCtas * 2 * g.nq * kRows);
+  l.part_o = take(sizeof(float) * static_cast<size_t>(kMaxCtas) * 2 * g.nq * kRows * g.dp);
+  if (!plan_in_cta(d, g)) {
+    l.pre = take(sizeof(int64_t) * (g.max_items + 1));
+    l.item = take(sizeof(int2) * g.max_items);
+    l.count = take(sizeof(int32_t));
+  }
+  l.total = at;
+  return l;
+}
+
+static bool encode(CUtensorMap* m, bool bf16, int rank, const void* base, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box) {
+  const EncodeFn fn = encode_fn();
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  return fn && fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                  const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K, typename... A>
+static cudaError_t launch(K kern, dim3 grid, int threads, size_t smem, cudaStream_t s, bool after_own, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_own ? 1 : 0;   // only behind this call's own kernels
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <class S, bool kBf16>
+static int run(const Params& P, const Geometry& g, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+               int dev, int sms, int kind, cudaStream_t s) {
+  const size_t smem = 1024 + S::kData + sizeof(Shared);
+  static_assert(1024 + S::kData + sizeof(Shared) <= kSmemMax, "shared memory");
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (!g_attr[dev][kind][kBf16]) {
+      if (cudaFuncSetAttribute(attention_kernel<S, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(smem)) != cudaSuccess)
+        return GR_ERR_CUDA;
+      g_attr[dev][kind][kBf16] = true;
+    }
+  }
+  const int ctas = sms < kMaxCtas ? sms : kMaxCtas;
+  if (P.pre &&
+      launch(plan_kernel<S::BN>, dim3(1), kPlanThreads, 0, s, false, P, S::NQ * P.tp, static_cast<int>(g.max_items)) !=
+          cudaSuccess)
+    return GR_ERR_CUDA;
+  if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, P.pre != nullptr, P, mq, mk, mv) !=
+      cudaSuccess)
+    return GR_ERR_CUDA;
+  if (ctas > 1 && launch(join_kernel<S::DP, S::NQ, kBf16>, dim3(ctas - 1, kJoinSlices), kJoinThreads, 0, s, true, P,
+                         ctas) != cudaSuccess)
+    return GR_ERR_CUDA;
+  return GR_OK;
+}
+
+}  // namespace grpa
+
+extern "C" int32_t gr_paged_attention_workspace_size(const gr_paged_attn_desc* d, size_t* bytes) {
+  using namespace grpa;
+  if (!bytes) return GR_ERR_NULL;
+  Geometry g;
+  const int rc = geometry(d, g);
+  if (rc != GR_OK) return rc;
+  *bytes = layout(d, g).total;
+  return GR_OK;
+}
+
+extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_paged_attn_io* io, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  gr::NvtxRange nvtx_range("gr_paged_attention");
+  using namespace grpa;
+  Geometry g;
+  int rc = geometry(d, g);
+  if (rc != GR_OK) return rc;
+  if (!io) return GR_ERR_NULL;
+  if ((io->beam_tail == nullptr) != (io->beam_steps == nullptr)) return GR_ERR_NULL;
+  if (io->beam_steps != nullptr && !d->causal) return GR_ERR_BAD_DESC;
+  if (d->num_seqs == 0 || d->num_tokens == 0) return GR_OK;
+  if (!io->q || !io->cu_seqlens || !io->seq_lens || !io->out || !workspace) return GR_ERR_NULL;
+  const bool keys = d->num_blocks > 0 && d->max_blocks > 0;
+  if (keys && (!io->k_cache || !io->v_cache || !io->block_table)) return GR_ERR_NULL;
+  const auto off16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
+  const auto off8 = [](int64_t a, int64_t n) { return n > 1 && (a % 8 != 0 || a <= 0 || a >= (1ll << 38)); };
+  if (off16(io->q) || off16(io->out) || (keys && (off16(io->k_cache) || off16(io->v_cache))) ||
+      off8(d->q_stride_tok, d->num_tokens) || off8(d->q_stride_head, d->num_heads) ||
+      off8(d->out_stride_tok, d->num_tokens) || off8(d->out_stride_head, d->num_heads) ||
+      off8(d->k_stride_block, d->num_blocks) || off8(d->k_stride_tok, d->block_size) ||
+      off8(d->k_stride_head, d->num_kv_heads) || off8(d->v_stride_block, d->num_blocks) ||
+      off8(d->v_stride_tok, d->block_size) || off8(d->v_stride_head, d->num_kv_heads))
+    return GR_ERR_MISALIGNED;
+  const Layout l = layout(d, g);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return GR_ERR_MISALIGNED;
+  if (workspace_bytes < l.total) return GR_ERR_WORKSPACE;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GR_ERR_NO_DEVICE;
+  {
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (g_sms[dev] == 0 && cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      g_sms[dev] = 0;
+      return GR_ERR_CUDA;
+    }
+    sms = g_sms[dev];
+  }
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  Params P;
+  P.table = io->block_table;
+  P.cu = io->cu_seqlens;
+  P.seq_lens = io->seq_lens;
+  P.tail = io->beam_tail;
+  P.steps = io->beam_steps;
+  P.out = io->out;
+  P.lse = io->lse;
+  P.err = io->err;
+  P.table_stride = d->table_stride;
+  P.num_blocks = d->num_blocks;
+  P.out_tok = d->out_stride_tok;
+  P.out_head = d->out_stride_head;
+  P.num_seqs = d->num_seqs;
+  P.num_tokens = d->num_tokens;
+  P.heads = d->num_heads;
+  P.kv_heads = d->num_kv_heads;
+  P.group = g.group;
+  P.dim = d->head_dim;
+  P.block_size = d->block_size;
+  P.max_blocks = keys ? d->max_blocks : 0;
+  P.causal = d->causal;
+  P.tp = g.tp;
+  P.box = g.box;
+  const char* stall = std::getenv("GR_TEST_STALL_COPIES");
+  P.flags = stall && stall[0] == '1' ? 1 : 0;
+  P.scale = d->scale;
+  P.scale_log2 = d->scale * gr::kLog2e;
+  P.hdr = reinterpret_cast<Hdr*>(ws + l.hdr);
+  P.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
+  P.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  P.pre = nullptr;
+  P.item = nullptr;
+  P.num_items = nullptr;
+  if (!plan_in_cta(d, g)) {
+    P.pre = reinterpret_cast<int64_t*>(ws + l.pre);
+    P.item = reinterpret_cast<int2*>(ws + l.item);
+    P.num_items = reinterpret_cast<int32_t*>(ws + l.count);
+  }
+  const bool bf16 = d->dtype == GR_DTYPE_BF16;
+  CUtensorMap mq, mk, mv;
+  // a dimension of one entry takes any legal stride
+  const auto bytes = [](int64_t stride, int64_t n) { return static_cast<cuuint64_t>(n > 1 ? stride * 2 : 16); };
+  {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d->head_dim), static_cast<cuuint64_t>(d->num_heads),
+                                static_cast<cuuint64_t>(d->num_tokens)};
+    const cuuint64_t str[2] = {bytes(d->q_stride_head, d->num_heads), bytes(d->q_stride_tok, d->num_tokens)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(g.group), static_cast<cuuint32_t>(g.tp)};
+    if (!encode(&mq, bf16, 3, io->q, dims, str, box)) return GR_ERR_CUDA;
+  }
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d->head_dim), static_cast<cuuint64_t>(d->num_kv_heads),
+                                static_cast<cuuint64_t>(d->block_size),
+                                static_cast<cuuint64_t>(keys ? d->num_blocks : 1)};
+    const cuuint64_t str[3] = {bytes(i ? d->v_stride_head : d->k_stride_head, d->num_kv_heads),
+                               bytes(i ? d->v_stride_tok : d->k_stride_tok, d->block_size),
+                               bytes(i ? d->v_stride_block : d->k_stride_block, keys ? d->num_blocks : 1)};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(g.box), 1};
+    // without keys no copy is in range: any readable address will do
+    const void* base = keys ? (i ? io->v_cache : io->k_cache) : io->q;
+    if (!encode(i ? &mv : &mk, bf16, 4, base, dims, str, box)) return GR_ERR_CUDA;
+  }
+  if (!keys) P.num_blocks = 1;   // the id behind the last block is 1: out of range
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const auto go = [&](auto shape, int kind) {
+    using S = decltype(shape);
+    return bf16 ? run<S, true>(P, g, mq, mk, mv, dev, sms, kind, s) : run<S, false>(P, g, mq, mk, mv, dev, sms, kind, s);
+  };
+  if (g.dp == 64) return g.nq == 1 ? go(Shape<64, 1>{}, 0) : go(Shape<64, 2>{}, 1);
+  if (g.dp == 128) return g.nq == 1 ? go(Shape<128, 1>{}, 2) : go(Shape<128, 2>{}, 3);
+  return go(Shape<256, 1>{}, 4);
+}
