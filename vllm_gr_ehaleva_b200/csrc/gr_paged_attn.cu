@@ -16,19 +16,19 @@
 // Single tokens use group rows of the 128; their product time hides behind the
 // cache reads, which bound them.
 //
-// Work.  A unit is one key tile of one (query block, KV head); the units of the
-// whole batch, in order, are cut into equal runs, one per CTA (one persistent
+// Work.  A (query block, KV head) of n key tiles costs n + kCost units; the
+// batch's units, in order, are cut into equal runs, one per CTA (one persistent
 // CTA per SM), whatever the lengths.  A (block, head) cut by a run's end leaves
 // partial outputs and log-sums in the workspace, joined by a second, small
 // kernel in a fixed order.  The prefix sums of the units come from a plan: up to
-// 128 query blocks are planned by every CTA for itself, more by a one-CTA kernel
+// 96 query blocks are planned by every CTA for itself, more by a one-CTA kernel
 // ahead.  For beams, key tiles between the tail and the block's first beam hold
 // only other beams' tokens and are not visited.
 //
-// Kernel.  Warp 0 loads (tensor-map copies of the blocks' rows, 128-byte
+// Kernel.  Warps 0 and 2 load (tensor-map copies of the blocks' rows, 128-byte
 // swizzle, a ring of key and value tiles), warp 1 issues the matrix products
-// (S = Q K^T from shared memory, O += P V with P in tensor memory), warp 2 owns
-// the tensor memory, warp 3 the plan; warps 4.. are the softmax: one thread per
+// (S = Q K^T from shared memory, O += P V with P in tensor memory), warp 3 walks
+// the run and hands out its (block, head) pairs; warps 4.. are the softmax: one thread per
 // row.  Two query tiles (kNQ = 2) have a softmax group each and alternate on the
 // tensor pipe; one tile (kNQ = 1: blocks of at most 128 rows, or heads above
 // 128) alternates two score buffers instead.
@@ -55,7 +55,12 @@ using gr::smem_u32;
 
 constexpr int kRows = 128;            // rows of a query tile (the matrix product's M)
 constexpr int kMaxCtas = 160;
-constexpr int kSmemPlan = 128;        // query blocks that a CTA plans for itself
+constexpr int kSmemPlan = 96;         // query blocks that a CTA plans for itself
+constexpr int kWorkRing = 4;          // (block, head) pairs handed out ahead
+#ifndef GR_PA_COST
+#define GR_PA_COST 2
+#endif
+constexpr int kCost = GR_PA_COST;     // what a (block, head) costs besides its key tiles, in key tiles
 constexpr int kSmemMax = 232448;      // shared memory a CTA may have
 constexpr float kRescale = 8.0f;      // log2 of the growth of the maximum that is let stand
 
@@ -76,8 +81,23 @@ struct Shape {
   static_assert(kColO + NQ * DP <= 512, "tensor memory columns");
 };
 
+// A (block, head) of a CTA's run, from the scheduling warp to the others.
+struct Work {
+  int req, q0;             // request, its first query token
+  int len, ctx;            // its keys, the position of its query token 0
+  int tail, steps;         // its beams
+  int t0, nt;              // the block's query tokens, from t0 of the request
+  int kvh;                 // KV head
+  int ta, tb, n;           // its key tiles: [0, ta) and from tb on, n in all
+  int j0, j1;              // those of the run
+  int slots;               // query tiles with rows; 0: the run is over
+  int pad;
+};
+
 struct Shared {
   uint64_t full[12], empty[12];
+  uint64_t wk_full[kWorkRing], wk_empty[kWorkRing];
+  Work work[kWorkRing];
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_full[2];   // scores ready / probabilities ready
   uint64_t pv_done[2], o_free[2];  // product into O finished / O read out
@@ -90,10 +110,10 @@ struct Shared {
 };
 
 struct Hdr {                       // a CTA's run, for the join
-  int64_t u0;                      // its first unit
-  int64_t beg, end;                // unit range of the (block, head) it starts in
+  int64_t u0;                      // where it starts, in cost units
+  int64_t beg, end;                // cost range of the (block, head) it starts in
   int32_t tok0, ntok;              // that block's query tokens
-  int32_t kvh, mid;                // its KV head; whether the run starts inside it
+  int32_t kvh, mid;                // its KV head; whether the run starts inside its key tiles
 };
 
 struct Params {
@@ -300,7 +320,7 @@ __device__ void plan_warp(const Params& P, Shared* sh) {
     if (i < items) {
       const int r = sh->item[i] & 255, b = sh->item[i] >> 8;
       const Seq s = load_seq(P, r);
-      u = static_cast<int64_t>(key_tiles<S::BN>(s, P.causal, b * per, min(s.n, (b + 1) * per)).n) * P.kv_heads;
+      u = static_cast<int64_t>(key_tiles<S::BN>(s, P.causal, b * per, min(s.n, (b + 1) * per)).n + kCost) * P.kv_heads;
     }
     const int64_t inc = warp_scan(u);
     if (i < items) sh->pre[i] = units + inc - u;
@@ -355,7 +375,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
     if (i < items) {
       const int2 it = P.item[i];
       const Seq s = load_seq(P, it.x);
-      u = static_cast<int64_t>(key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n) * P.kv_heads;
+      u = static_cast<int64_t>(key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n + kCost) * P.kv_heads;
     }
     const int64_t ex = block_scan(u, total, part);
     if (i < items) P.pre[i] = units + ex;
@@ -367,69 +387,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
   }
 }
 
-// A CTA's run of units and the (block, head) pairs in it, walked alike by every role.
-struct Walk {
-  const int64_t* pre;
-  int items, i;
-  int64_t u, end;
-};
-
-struct Work {
-  Seq s;
-  int t0, nt;        // query tokens of the block, from t0 of the request
-  int kvh;
-  Tiles tiles;
-  int j0, j1;        // key tiles of the run
-  int slots;         // query tiles with rows
-  int64_t beg;       // unit range of the (block, head)
-};
-
-template <class S>
-__device__ __forceinline__ Walk walk_begin(const Params& P, const Shared* sh, int cta, int ctas) {
-  Walk w;
-  w.pre = P.pre ? P.pre : sh->pre;
-  w.items = P.pre ? P.num_items[0] : sh->num_items;
-  const int64_t units = w.pre[w.items];
-  w.u = units * cta / ctas;
-  w.end = units * (cta + 1) / ctas;
-  int lo = 0, hi = w.items > 0 ? w.items - 1 : 0;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (w.pre[mid] <= w.u) lo = mid; else hi = mid - 1;
-  }
-  w.i = lo;
-  return w;
-}
-
-template <class S>
-__device__ __forceinline__ bool walk_next(const Params& P, const Shared* sh, Walk& w, Work& k) {
-  if (w.u >= w.end) return false;
-  while (w.pre[w.i + 1] <= w.u) ++w.i;
-  int r, b;
-  if (P.pre) {
-    const int2 it = P.item[w.i];
-    r = it.x;
-    b = it.y;
-  } else {
-    r = sh->item[w.i] & 255;
-    b = sh->item[w.i] >> 8;
-  }
-  const int per = S::NQ * P.tp;
-  k.s = load_seq(P, r);
-  k.t0 = b * per;
-  k.nt = min(k.s.n - k.t0, per);
-  k.tiles = key_tiles<S::BN>(k.s, P.causal, k.t0, k.t0 + k.nt);
-  const int64_t in = w.u - w.pre[w.i];
-  k.kvh = static_cast<int>(in / k.tiles.n);
-  k.j0 = static_cast<int>(in - static_cast<int64_t>(k.kvh) * k.tiles.n);
-  k.j1 = static_cast<int>(min(static_cast<int64_t>(k.tiles.n), k.j0 + (w.end - w.u)));
-  k.slots = k.nt > P.tp ? 2 : 1;
-  k.beg = w.u - k.j0;
-  w.u += k.j1 - k.j0;
-  return true;
-}
-
-__device__ __forceinline__ int tile_at(const Tiles& t, int j) { return j < t.a ? j : j - t.a + t.b; }
+__device__ __forceinline__ int tile_at(const Work& k, int j) { return j < k.ta ? j : j - k.ta + k.tb; }
 
 // ---------------------------------------------------------------- roles
 template <class S>
@@ -444,78 +402,181 @@ struct Ring {        // position in the ring of key and value tiles
   }
 };
 
-// Warp 0: the block's queries once, then its key and value tiles in the order
-// in which the matrix products first use them.
+// The next (block, head) of the run; false at its end or when a wait gave up.
+__device__ __forceinline__ bool next_work(Shared* sh, uint32_t& seq, Work& k) {
+  const int at = seq % kWorkRing;
+  if (!wait(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u)) return false;
+  k = sh->work[at];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->wk_empty[at]);
+  ++seq;
+  return k.slots > 0;
+}
+
+// Warp 3: walks the CTA's run [cost * cta / ctas, cost * (cta + 1) / ctas) of the
+// batch's cost and hands out its (block, head) pairs ahead of their use.  A pair
+// of n key tiles spans kCost + n units: a border in the first kCost leaves it
+// whole, a border behind cuts its key tiles.  Also the header for the join.
+template <class S>
+__device__ __forceinline__ void schedule_role(const Params& P, Shared* sh, int ctas) {
+  const int lane = threadIdx.x & 31;
+  const int64_t* pre = P.pre ? P.pre : sh->pre;
+  const int items = P.pre ? P.num_items[0] : sh->num_items;
+  const int64_t units = pre[items];
+  Hdr h{units, 0, 0, 0, 0, 0, 0};
+  if (static_cast<int>(blockIdx.x) >= ctas) {
+    if (lane == 0) P.hdr[blockIdx.x] = h;
+    return;
+  }
+  int64_t u = units * blockIdx.x / ctas;
+  const int64_t end = units * (blockIdx.x + 1) / ctas;
+  h.u0 = u;
+  int lo = 0, hi = items - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  const int per = S::NQ * P.tp;
+  bool first = true;
+  uint32_t seq = 0;
+  for (int i = lo; u < end; ++i) {
+    int r, b;
+    if (P.pre) {
+      const int2 it = P.item[i];
+      r = it.x;
+      b = it.y;
+    } else {
+      r = sh->item[i] & 255;
+      b = sh->item[i] >> 8;
+    }
+    const Seq s = load_seq(P, r);
+    Work k;
+    k.req = r;
+    k.q0 = s.q0;
+    k.len = s.len;
+    k.ctx = s.ctx;
+    k.tail = s.tail;
+    k.steps = s.steps;
+    k.t0 = b * per;
+    k.nt = min(s.n - k.t0, per);
+    k.slots = k.nt > P.tp ? 2 : 1;
+    k.pad = 0;
+    const Tiles t = key_tiles<S::BN>(s, P.causal, k.t0, k.t0 + k.nt);
+    k.ta = t.a;
+    k.tb = t.b;
+    k.n = t.n;
+    const int span = t.n + kCost;
+    const int64_t in = u - pre[i];
+    int off = 0;
+    k.kvh = 0;
+    if (in > 0) {
+      k.kvh = static_cast<int>(in / span);
+      off = static_cast<int>(in - static_cast<int64_t>(k.kvh) * span);
+    }
+    for (; k.kvh < P.kv_heads && u < end; ++k.kvh, off = 0) {
+      const int64_t beg = u - off;
+      const int stop = static_cast<int>(min(static_cast<int64_t>(span), off + (end - u)));
+      k.j0 = max(off - kCost, 0);
+      k.j1 = max(stop - kCost, 0);
+      u += stop - off;
+      if (first) {
+        first = false;
+        h.beg = beg;
+        h.end = beg + span;
+        h.tok0 = s.q0 + k.t0;
+        h.ntok = k.nt;
+        h.kvh = k.kvh;
+        h.mid = k.j0 > 0;
+        if (lane == 0) P.hdr[blockIdx.x] = h;
+      }
+      if (k.j1 <= k.j0) continue;
+      const int at = seq % kWorkRing;
+      if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
+      if (lane == 0) {
+        sh->work[at] = k;
+        mbar_arrive(&sh->wk_full[at]);
+      }
+      ++seq;
+    }
+  }
+  const int at = seq % kWorkRing;
+  if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
+  if (lane == 0) {
+    sh->work[at].slots = 0;
+    mbar_arrive(&sh->wk_full[at]);
+  }
+}
+
+// Warps 0 and 2: the block's queries once (warp 0), then its key and value tiles
+// in the order in which the matrix products first use them, half of a tile's
+// copies each (blocks of 16 rows make 32 copies of a key and a value tile: one
+// warp cannot issue them at the rate of the memory).
 template <class S>
 __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t data, const CUtensorMap* mq,
-                                          const CUtensorMap* mk, const CUtensorMap* mv, int ctas) {
+                                          const CUtensorMap* mk, const CUtensorMap* mv, int half) {
   const int lane = threadIdx.x & 31;
-  Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
   Work k;
   Ring<S> ring;
-  uint32_t qphase = 0;
+  uint32_t qphase = 0, seq = 0;
   int64_t issued = 0;
   bool q_issued = false, ok = true;
   const uint32_t ringbase = data + S::NQ * S::kQTile;
   const int boxes = S::BN / P.box;
+  // this lane's copy of a tile: column chunk c of box bx
+  const int per = (boxes * S::CH + 1) / 2;
+  const int e = half * per + lane, bx = e / S::CH, c = e - bx * S::CH;
+  const bool mine = lane < per && bx < boxes;
+  const uint32_t at = c * S::kChunkKV + bx * P.box * 128;
   const int oob = static_cast<int>(P.num_blocks);
   int bad = 0;
-  while (ok && walk_next<S>(P, sh, w, k)) {
-    if (!wait(sh, &sh->q_empty, qphase ^ 1u)) { ok = false; break; }
-    if (lane == 0) {
-      const int slots = S::NQ == 2 ? k.slots : 1;
-      const uint32_t bytes = static_cast<uint32_t>(slots * S::CH * P.group * P.tp * 128);
-      if (!(P.flags & 1)) {
-        mbar_arrive_expect_tx(&sh->q_full, bytes);
+  while (ok && next_work(sh, seq, k)) {
+    if (half == 0) {
+      if (!wait(sh, &sh->q_empty, qphase ^ 1u)) {
+        ok = false;
+        break;
+      }
+      if (lane == 0 && !(P.flags & 1)) {
+        const int slots = S::NQ == 2 ? k.slots : 1;
+        mbar_arrive_expect_tx(&sh->q_full, static_cast<uint32_t>(slots * S::CH * P.group * P.tp * 128));
         for (int q = 0; q < slots; ++q)
-          for (int c = 0; c < S::CH; ++c)
-            tma_load3(data + q * S::kQTile + c * S::kChunkQ, mq, c * 64, k.kvh * P.group, k.s.q0 + k.t0 + q * P.tp,
+          for (int x = 0; x < S::CH; ++x)
+            tma_load3(data + q * S::kQTile + x * S::kChunkQ, mq, x * 64, k.kvh * P.group, k.q0 + k.t0 + q * P.tp,
                       &sh->q_full);
         q_issued = true;
       }
+      qphase ^= 1u;
     }
-    qphase ^= 1u;
     const int n = k.j1 - k.j0;
     const int lead = S::NQ == 2 ? 1 : 2;
-    const int req_row = P.pre ? P.item[w.i].x : (sh->item[w.i] & 255);
-    const int32_t* row = P.table + req_row * P.table_stride;
+    const int32_t* row = P.table + k.req * P.table_stride;
     // the order K0 .. K(lead-1), V0, K(lead), V1, ...
     for (int x = 0, ki = 0, vi = 0; x < 2 * n; ++x) {
       const bool is_k = ki < n && ki < vi + lead;
       const int j = is_k ? ki++ : vi++;
-      const int key0 = tile_at(k.tiles, k.j0 + j) * S::BN;
-      // this lane's boxes: the block ids first, so that their latency overlaps the wait
-      int id[2] = {oob, oob};   // box at lane, at lane + 32 (BN / 8 * CH <= 64)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int bx = (lane + 32 * h) / S::CH;
-        const int tok = key0 + bx * P.box;
-        if (bx < boxes && tok < k.s.len) {
-          const int v = __ldg(row + tok / P.block_size);
-          if (v < 0 || v >= oob) bad = 1; else id[h] = v;
-        }
+      // the block id first, so that its latency overlaps the wait
+      const int tok = tile_at(k, k.j0 + j) * S::BN + bx * P.box;
+      int id = oob;
+      if (mine && tok < k.len) {
+        const int v = __ldg(row + tok / P.block_size);
+        if (v < 0 || v >= oob) bad = 1; else id = v;
       }
-      if (!wait(sh, &sh->empty[ring.stage], ring.phase ^ 1u)) { ok = false; break; }
+      if (!wait(sh, &sh->empty[ring.stage], ring.phase ^ 1u)) {
+        ok = false;
+        break;
+      }
       if (!(P.flags & 1)) {
-        if (lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
+        if (half == 0 && lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
         __syncwarp();
-        const uint32_t dst = ringbase + ring.stage * S::kStage;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int e = lane + 32 * h, bx = e / S::CH, c = e % S::CH;
-          if (bx < boxes) {
-            const int tok = key0 + bx * P.box;
-            tma_load4(dst + c * S::kChunkKV + bx * P.box * 128, is_k ? mk : mv, c * 64, k.kvh, tok % P.block_size, id[h],
-                      &sh->full[ring.stage]);
-          }
-        }
+        if (mine)
+          tma_load4(ringbase + ring.stage * S::kStage + at, is_k ? mk : mv, c * 64, k.kvh, tok % P.block_size, id,
+                    &sh->full[ring.stage]);
         ++issued;
       }
       ring.next();
     }
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_SLOT);
-  if (!ok) {
+  if (*reinterpret_cast<volatile int*>(&sh->abort)) {
     // gave up: wait (bounded) for the copies in flight before the shared memory goes
     int64_t left = issued < S::kStages ? issued : S::kStages;
     for (; left > 0; --left) {
@@ -546,7 +607,7 @@ __device__ __forceinline__ void zero_tail(uint32_t tile, int from, int to) {
 
 // Warp 1: the matrix products, issued by one lane.
 template <class S, bool kBf16>
-__device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t data, int ctas) {
+__device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t data) {
   const int lane = threadIdx.x & 31;
   const uint32_t tmem = sh->tmem;
   const uint32_t ringbase = data + S::NQ * S::kQTile;
@@ -585,12 +646,11 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
     __syncwarp();
   };
 
-  Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
   Work k;
   Ring<S> ring;
-  uint32_t qphase = 0, pphase = 0, ofree = 3;   // one bit per buffer / tile
+  uint32_t seq = 0, qphase = 0, pphase = 0, ofree = 3;   // one bit per buffer / tile
   uint32_t step = 0;    // score buffer of the next step (kNQ = 1)
-  while (walk_next<S>(P, sh, w, k)) {
+  while (next_work(sh, seq, k)) {
     const int n = k.j1 - k.j0;
     if (!wait(sh, &sh->q_full, qphase)) return;
     qphase ^= 1u;
@@ -604,8 +664,7 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
     };
     const auto take_v = [&](int& stage, int j) {
       if (!take(stage)) return false;
-      const int key0 = tile_at(k.tiles, k.j0 + j) * S::BN;
-      const int live = k.s.len - key0;
+      const int live = k.len - tile_at(k, k.j0 + j) * S::BN;
       if (live > 0 && live < S::BN && live % P.box != 0)
         zero_tail<S>(ringbase + stage * S::kStage, live, (live / P.box + 1) * P.box);
       return true;
@@ -672,7 +731,7 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
 // Warps 4..: softmax of one query tile, one thread per row; also the rare
 // rescaling of the accumulator, and the block's output.
 template <class S, bool kBf16>
-__device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int slot, int ctas) {
+__device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int slot) {
   constexpr int BN = S::BN, DP = S::DP;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
   const int m_row = warp * 32 + lane;
@@ -681,29 +740,28 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
   const uint32_t o_col = tmem + S::kColO + slot * DP;
   const float c = P.scale_log2;
   const int ti = m_row / P.group, g = m_row - ti * P.group;
-  Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
   Work k;
-  uint32_t sphase = 0, pvphase = 0;   // one bit per buffer
+  uint32_t seq = 0, sphase = 0, pvphase = 0;   // one bit per buffer
   uint32_t step = 0;
-  while (walk_next<S>(P, sh, w, k)) {
+  while (next_work(sh, seq, k)) {
     if (S::NQ == 2 && slot >= k.slots) continue;
     const int n = k.j1 - k.j0;
     // this row: token, position, the keys it sees
     const int tok = k.t0 + slot * P.tp + ti;              // in the request
     const bool live = ti < P.tp && ti + slot * P.tp < k.nt;
-    const int pos = k.s.ctx + tok;
-    int lim = P.causal ? min(pos + 1, k.s.len) : k.s.len;
+    const int pos = k.ctx + tok;
+    int lim = P.causal ? min(pos + 1, k.len) : k.len;
     int first = 0x7FFFFFFF, own = 0;
-    if (k.s.steps > 0 && tok >= k.s.tail) {
-      first = k.s.ctx + k.s.tail;
-      own = first + (tok - k.s.tail) / k.s.steps * k.s.steps;
+    if (k.steps > 0 && tok >= k.tail) {
+      first = k.ctx + k.tail;
+      own = first + (tok - k.tail) / k.steps * k.steps;
     }
     if (!live) lim = 0x7FFFFFFF, first = 0x7FFFFFFF;      // rows of no token: no mask, nothing stored
     const bool any_live = __any_sync(0xFFFFFFFFu, live);
     float m = -kInf, l = 0.0f;
     for (int j = 0; j < n; ++j) {
       const int b = S::NQ == 2 ? slot : static_cast<int>((step + j) & 1);
-      const int key0 = tile_at(k.tiles, k.j0 + j) * BN;
+      const int key0 = tile_at(k, k.j0 + j) * BN;
       if (!wait(sh, &sh->s_full[b], (sphase >> b) & 1u)) return;
       sphase ^= 1u << b;
       tc_fence_after();
@@ -793,11 +851,11 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
     if (!wait(sh, &sh->pv_done[lb], ((pvphase >> lb) & 1u) ^ 1u)) return;
     tc_fence_after();
     if (S::NQ == 1) step += n;
-    const bool whole = k.j0 == 0 && k.j1 == k.tiles.n;
+    const bool whole = k.j0 == 0 && k.j1 == k.n;
     if (any_live) {
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       const float lse2 = l > 0.0f || l != l ? m * c + __log2f(l) : -kInf;
-      const int64_t t = static_cast<int64_t>(k.s.q0) + tok;
+      const int64_t t = static_cast<int64_t>(k.q0) + tok;
       const int h = k.kvh * P.group + g;
       const int part = blockIdx.x * 2 + (k.j0 == 0 ? 1 : 0);
       const int prow = slot * kRows + m_row;
@@ -857,6 +915,10 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       mbar_init(&sh->full[i], 1);
       mbar_init(&sh->empty[i], 1);
     }
+    for (int i = 0; i < kWorkRing; ++i) {
+      mbar_init(&sh->wk_full[i], 1);
+      mbar_init(&sh->wk_empty[i], 3 + 4 * S::NQ);
+    }
     mbar_init(&sh->q_full, 1);
     mbar_init(&sh->q_empty, 1);
     mbar_init(&sh->drain, 1);
@@ -885,25 +947,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   const int64_t units = P.pre ? P.pre[P.num_items[0]] : sh->pre[sh->num_items];
   const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), units));
   const bool busy = static_cast<int>(blockIdx.x) < ctas;
-  if (warp == 3) {
-    // the run's header for the join, and the requests' lengths checked once
-    if (lane == 0) {
-      Hdr h{units, 0, 0, 0, 0, 0, 0};
-      if (busy) {
-        Walk w = walk_begin<S>(P, sh, blockIdx.x, ctas);
-        Work k;
-        h.u0 = w.u;
-        if (walk_next<S>(P, sh, w, k)) {
-          h.beg = k.beg;
-          h.end = k.beg + k.tiles.n;
-          h.tok0 = k.s.q0 + k.t0;
-          h.ntok = k.nt;
-          h.kvh = k.kvh;
-          h.mid = k.j0 > 0;
-        }
-      }
-      P.hdr[blockIdx.x] = h;
-    }
+  if (warp == 3) {   // the requests' lengths, checked once
     int bad = 0;
     for (int r = blockIdx.x * 32 + lane; r < P.num_seqs; r += gridDim.x * 32) load_seq(P, r, &bad);
     if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_RECORD);
@@ -911,10 +955,12 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   // registers of the two-tile kernel: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168, what the launch has
   if (warp < 4) {
     if constexpr (S::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0 && busy) {
-      load_role<S>(P, sh, base, &mq, &mk, &mv, ctas);
+    if (warp == 3) {
+      schedule_role<S>(P, sh, ctas);
+    } else if (warp != 1 && busy) {
+      load_role<S>(P, sh, base, &mq, &mk, &mv, warp >> 1);
     } else if (warp == 1 && busy) {
-      mma_role<S, kBf16>(P, sh, base, ctas);
+      mma_role<S, kBf16>(P, sh, base);
       if (sh->abort) {   // products in flight finish before the tensor memory goes
         if (lane == 0) tc_commit(&sh->drain);
         __syncwarp();
@@ -923,7 +969,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     }
   } else {
     if constexpr (S::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    if (busy) softmax_role<S, kBf16>(P, sh, (warp >> 2) - 1, ctas);
+    if (busy) softmax_role<S, kBf16>(P, sh, (warp >> 2) - 1);
   }
   __syncwarp();
   tc_fence_before();
@@ -946,7 +992,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int 
   gr::pdl_wait();
   const int c = blockIdx.x + 1;
   const Hdr h = P.hdr[c];
-  if (!h.mid || P.hdr[c - 1].u0 > h.beg) return;
+  if (!h.mid || P.hdr[c - 1].u0 > h.beg + kCost) return;
   int last = c;                              // the last run with a part of it
   while (last + 1 < ctas && P.hdr[last + 1].u0 < h.end) ++last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
