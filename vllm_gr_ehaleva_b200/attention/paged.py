@@ -29,14 +29,19 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _I32, _I64 = torch.int32, torch.int64
 
 
+# the current stream's handle by device index, without a Stream object around it
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(fn, name, device, *args):
     """Calls an entry point on the device's current stream, with the device current."""
     index = device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, _stream(index))
     if rc != _lib.GR_OK:
         raise RuntimeError(f"{name} failed: {_lib.STATUS_NAMES.get(rc, rc)}")
 
@@ -109,11 +114,12 @@ def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_s
     lib = _lib.load()
     ints = torch.empty(2 * R + 2, dtype=_I32, device=device)
     longs = torch.empty((2, n), dtype=_I64, device=device)
-    cu, lens, used = ints[:R + 1], ints[R + 1:2 * R + 1], ints[2 * R + 1:]
-    at = ints.data_ptr()
+    at, to = ints.data_ptr(), longs.data_ptr()
     _call(lib.gr_extend_block_tables, "gr_extend_block_tables", device, d, table, cached, fresh, free, at,
-          at + 4 * (R + 1), longs.data_ptr(), longs.data_ptr() + 8 * n, at + 4 * (2 * R + 1), err)
-    return {"cu_seqlens_q": cu, "seq_lens": lens, "slot_mapping": longs[0], "positions": longs[1], "blocks_used": used}
+          at + 4 * (R + 1), to, to + 8 * n, at + 4 * (2 * R + 1), err)
+    cu, lens, used = ints.split_with_sizes((R + 1, R, 1))
+    slots, positions = longs.unbind(0)
+    return {"cu_seqlens_q": cu, "seq_lens": lens, "slot_mapping": slots, "positions": positions, "blocks_used": used}
 
 
 def _check_caches(k_cache, v_cache):

@@ -982,28 +982,38 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 }
 
 // ---------------------------------------------------------------- join
-// One CTA row of the grid per run boundary: the first boundary inside a (block,
-// head) joins all its parts, in run order, with weights 2^(lse_i - max).
-constexpr int kJoinThreads = 128;
-constexpr int kJoinSlices = 4;
+// One grid column per run border: the first border inside a (block, head) joins
+// all its parts, in run order, with weights 2^(lse_i - max); a warp per row.
+// The headers, the parts' log-sums and then up to four parts' rows at a time are
+// loaded together: the kernel is a few memory latencies long.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
 
 template <int DP, int NQ, bool kBf16>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int ctas) {
   gr::pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x + 1;
   const Hdr h = P.hdr[c];
-  if (!h.mid || P.hdr[c - 1].u0 > h.beg + kCost) return;
-  int last = c;                              // the last run with a part of it
-  while (last + 1 < ctas && P.hdr[last + 1].u0 < h.end) ++last;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t before = P.hdr[c - 1].u0;
+  int parts = 2;                             // runs c - 1, c and those behind that start in the pair
+  for (int i = c + 1;; i += 32) {
+    const bool in = i + lane < ctas && P.hdr[min(i + lane, ctas - 1)].u0 < h.end;
+    const int n = __popc(__ballot_sync(0xFFFFFFFFu, in));
+    parts += n;
+    if (n < 32) break;
+  }
+  if (!h.mid || before > h.beg + kCost) return;
   const int rows = h.ntok * P.group;
-  for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows; r += kJoinSlices * (kJoinThreads / 32)) {
+  for (int r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
     const int tok = r / P.group, g = r - tok * P.group;
     const int slot = tok / P.tp;
     const int prow = slot * kRows + (tok - slot * P.tp) * P.group + g;
-    const auto at = [&](int i) { return static_cast<int64_t>(i * 2 + (i == c - 1 ? 1 : 0)) * NQ * kRows + prow; };
-    float top = -kInf;
-    for (int i = c - 1 + lane; i <= last; i += 32) top = fmaxf(top, P.part_lse[at(i)]);
+    // the first part lies in its run's second place, the others in their first
+    const auto at = [&](int i) { return static_cast<int64_t>((c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * NQ * kRows + prow; };
+    const float mine = lane < parts ? P.part_lse[at(lane)] : -kInf;
+    float top = mine;
+    for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, P.part_lse[at(i)]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float ref = top == -kInf ? 0.0f : top;
@@ -1011,15 +1021,27 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int 
 #pragma unroll
     for (int x = 0; x < DP / 32; ++x) acc[x] = 0.0f;
     float sum = 0.0f;
-    for (int i = c - 1; i <= last; ++i) {
-      const float wgt = gr::fast_exp2(P.part_lse[at(i)] - ref);
-      const float* o = P.part_o + at(i) * DP;
-      sum += wgt;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const float w = gr::fast_exp2((i0 == 0 ? mine : (i0 + lane < parts ? P.part_lse[at(i0 + lane)] : -kInf)) - ref);
+      const int n = min(32, parts - i0);
+      for (int i = 0; i < n; i += 4) {
+        float2 v[4][DP / 64];
 #pragma unroll
-      for (int x = 0; x < DP / 64; ++x) {
-        const float2 v = *reinterpret_cast<const float2*>(o + x * 64 + lane * 2);
-        acc[2 * x] += wgt * v.x;
-        acc[2 * x + 1] += wgt * v.y;
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x)
+            v[y][x] = i + y < n ? *reinterpret_cast<const float2*>(P.part_o + at(i0 + i + y) * DP + x * 64 + lane * 2)
+                                : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float wy = __shfl_sync(0xFFFFFFFFu, w, i + y);   // 0 behind the last part
+          sum += i + y < n ? wy : 0.0f;
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x) {
+            acc[2 * x] += wy * v[y][x].x;
+            acc[2 * x + 1] += wy * v[y][x].y;
+          }
+        }
       }
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
@@ -1060,7 +1082,7 @@ static EncodeFn encode_fn() {
 }
 
 struct Geometry {
-  int dp, nq, bn, group, tp, box;
+  int dp, nq, bn, group, tp, box, longest;
   int64_t max_items;
 };
 
@@ -1083,6 +1105,7 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
   g.bn = g.dp == 256 ? 64 : 128;
   g.box = 8;
   while (g.box * 2 <= g.bn && d->block_size % (g.box * 2) == 0) g.box *= 2;
+  g.longest = d->max_query_len > 0 ? d->max_query_len : 1;
   const int64_t per = static_cast<int64_t>(g.nq) * g.tp;
   g.max_items = static_cast<int64_t>(d->num_tokens) / per + d->num_seqs;
   if (g.max_items > 0x7FFFFFFF) return GR_ERR_UNSUPPORTED;
@@ -1165,7 +1188,10 @@ static int run(const Params& P, const Geometry& g, const CUtensorMap& mq, const 
   if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, P.pre != nullptr, P, mq, mk, mv) !=
       cudaSuccess)
     return GR_ERR_CUDA;
-  if (ctas > 1 && launch(join_kernel<S::DP, S::NQ, kBf16>, dim3(ctas - 1, kJoinSlices), kJoinThreads, 0, s, true, P,
+  // two rows of a block per warp of the join
+  const int64_t rows = static_cast<int64_t>(g.longest < S::NQ * g.tp ? g.longest : S::NQ * g.tp) * g.group;
+  const int slices = static_cast<int>((rows + 2 * kJoinWarps - 1) / (2 * kJoinWarps));
+  if (ctas > 1 && launch(join_kernel<S::DP, S::NQ, kBf16>, dim3(ctas - 1, slices), kJoinThreads, 0, s, true, P,
                          ctas) != cudaSuccess)
     return GR_ERR_CUDA;
   return GR_OK;

@@ -46,6 +46,12 @@ struct TableParams {
   int num_seqs, num_tokens, num_free, block_size, max_blocks;
 };
 
+// Blocks of `tokens` (at most 2^31 - 1) tokens; 32-bit arithmetic, a 64-bit division is a
+// subroutine several times as long.
+__device__ __forceinline__ int blocks_of(int tokens, int bs) {
+  return static_cast<int>((static_cast<uint32_t>(tokens) + static_cast<uint32_t>(bs) - 1u) / static_cast<uint32_t>(bs));
+}
+
 __device__ __forceinline__ int clamp32(int64_t v) { return v > 0x7FFFFFFF ? 0x7FFFFFFF : static_cast<int>(v); }
 
 // Exclusive sums over the CTA's threads of two values; totals in t0 / t1.
@@ -100,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) extend_block_tables_kernel(const Tab
   int bad = 0;
   for (int r0 = 0; r0 < P.num_seqs; r0 += kTile) {
     const int nr = min(kTile, P.num_seqs - r0);
-    int c[kPerThread], f[kPerThread];
+    int c[kPerThread], f[kPerThread], take[kPerThread];
     int64_t a = 0, b = 0;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
@@ -115,8 +121,9 @@ __global__ void __launch_bounds__(kThreads) extend_block_tables_kernel(const Tab
           f[i] = 0;
         }
       }
+      take[i] = blocks_of(c[i] + f[i], bs) - blocks_of(c[i], bs);
       a += f[i];
-      b += (static_cast<int64_t>(c[i]) + f[i] + bs - 1) / bs - (static_cast<int64_t>(c[i]) + bs - 1) / bs;
+      b += take[i];
     }
     int64_t ta, tb;
     scan2(a, b, ta, tb, s_part);
@@ -127,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) extend_block_tables_kernel(const Tab
       s_base[r] = blk0 + b;
       s_cached[r] = c[i];
       a += f[i];
-      b += (static_cast<int64_t>(c[i]) + f[i] + bs - 1) / bs - (static_cast<int64_t>(c[i]) + bs - 1) / bs;
+      b += take[i];
     }
     if (threadIdx.x == 0) {
       s_cu[kTile] = tok0 + ta;
@@ -143,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) extend_block_tables_kernel(const Tab
     const int64_t eb = blk0 + tb * me / G, ee = blk0 + tb * (me + 1) / G;
     for (int64_t e = eb + threadIdx.x; e < ee; e += kThreads) {
       const int r = last_le(s_base, nr, e);
-      const int64_t j = (static_cast<int64_t>(s_cached[r]) + bs - 1) / bs + (e - s_base[r]);
+      const int64_t j = blocks_of(s_cached[r], bs) + (e - s_base[r]);
       if (e < P.num_free && j < P.max_blocks)
         P.table[(r0 + r) * P.table_stride + j] = P.free_blocks[e];
       else
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) extend_block_tables_kernel(const Tab
       const int r = last_le(s_cu, nr, t);
       const int cach = s_cached[r];
       const int p = cach + static_cast<int>(t - s_cu[r]);
-      const int j = p / bs, have = static_cast<int>((static_cast<int64_t>(cach) + bs - 1) / bs);
+      const int j = p / bs, have = blocks_of(cach, bs);
       int id = -1;
       if (j < P.max_blocks) {
         if (j < have) {
