@@ -130,6 +130,7 @@ struct Params {
   int block_size, max_blocks, causal;
   int tp;                          // query tokens per tile
   int box;                         // rows of a block that one copy takes
+  int out32;                       // output rows start on 32 bytes
   int flags;                       // 1: copies are not issued (test hook)
   float scale_log2, scale;
   // plan and partials in the workspace
@@ -137,7 +138,7 @@ struct Params {
   int2* item;                      // request, block
   int32_t* num_items;
   Hdr* hdr;
-  float* part_o;                   // [ctas][2][NQ * 128][DP]
+  float4* part_o;                  // [ctas][2][NQ][DP / 4][128 rows]: a warp's stores of its 32 rows are whole lines
   float* part_lse;                 // [ctas][2][NQ * 128]
 };
 
@@ -224,6 +225,12 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // A wait by a whole warp.  One that gives up sets the CTA's abort flag, which
@@ -867,7 +874,7 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
         }
       }
       unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
-      float* prt = P.part_o + (static_cast<int64_t>(part) * S::NQ * kRows + prow) * DP;
+      float4* prt = P.part_o + (static_cast<int64_t>(part) * S::NQ + slot) * (DP / 4) * kRows + m_row;
 #pragma unroll 1
       for (int x = 0; x < DP; x += 32) {
         uint32_t o[32];
@@ -876,20 +883,23 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
         if (live) {
           if (whole) {
 #pragma unroll
-            for (int y = 0; y < 32; y += 8) {
-              if (x + y < P.dim) {
-                uint4 v;
-                v.x = pack16<kBf16>(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv);
-                v.y = pack16<kBf16>(__uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
-                v.z = pack16<kBf16>(__uint_as_float(o[y + 4]) * inv, __uint_as_float(o[y + 5]) * inv);
-                v.w = pack16<kBf16>(__uint_as_float(o[y + 6]) * inv, __uint_as_float(o[y + 7]) * inv);
-                *reinterpret_cast<uint4*>(orow + (x + y) * 2) = v;
+            for (int y = 0; y < 32; y += 16) {
+              uint32_t v[8];
+#pragma unroll
+              for (int z = 0; z < 8; ++z)
+                v[z] = pack16<kBf16>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
+              unsigned char* to = orow + (x + y) * 2;
+              if (P.out32) {            // whole sectors; the head dim is a multiple of 16 then
+                if (x + y < P.dim) st_global_32(to, v);
+              } else {
+                if (x + y < P.dim) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+                if (x + y + 8 < P.dim) *reinterpret_cast<uint4*>(to + 16) = make_uint4(v[4], v[5], v[6], v[7]);
               }
             }
           } else {
 #pragma unroll
             for (int y = 0; y < 32; y += 4)
-              *reinterpret_cast<float4*>(prt + x + y) =
+              prt[(x + y) / 4 * kRows] =
                   make_float4(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv,
                               __uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
           }
@@ -983,11 +993,12 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 
 // ---------------------------------------------------------------- join
 // One grid column per run border: the first border inside a (block, head) joins
-// all its parts, in run order, with weights 2^(lse_i - max); a warp per row.
-// The headers, the parts' log-sums and then up to four parts' rows at a time are
-// loaded together: the kernel is a few memory latencies long.
+// all its parts, in run order, with weights 2^(lse_i - max).  A warp takes eight
+// rows, four lanes each; the headers, the log-sums and then up to four parts'
+// columns at a time are loaded together: the kernel is a few memory latencies long.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinRows = 8 * kJoinWarps;
 
 template <int DP, int NQ, bool kBf16>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int ctas) {
@@ -1005,56 +1016,63 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int 
   }
   if (!h.mid || before > h.beg + kCost) return;
   const int rows = h.ntok * P.group;
-  for (int r = blockIdx.y * kJoinWarps + warp; r < rows; r += gridDim.y * kJoinWarps) {
+  for (int r0 = blockIdx.y * kJoinRows + warp * 8; r0 < rows; r0 += gridDim.y * kJoinRows) {
+    const int r = min(r0 + (lane & 7), rows - 1), quarter = lane >> 3;
+    const bool live = r0 + (lane & 7) < rows;
     const int tok = r / P.group, g = r - tok * P.group;
     const int slot = tok / P.tp;
-    const int prow = slot * kRows + (tok - slot * P.tp) * P.group + g;
+    const int m_row = (tok - slot * P.tp) * P.group + g;
     // the first part lies in its run's second place, the others in their first
-    const auto at = [&](int i) { return static_cast<int64_t>((c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * NQ * kRows + prow; };
-    const float mine = lane < parts ? P.part_lse[at(lane)] : -kInf;
-    float top = mine;
-    for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, P.part_lse[at(i)]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const auto at = [&](int i) { return (static_cast<int64_t>(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * NQ + slot; };
+    // the row's four lanes share the log-sums
+    float top = -kInf;
+    for (int i = quarter; i < parts; i += 4) top = fmaxf(top, P.part_lse[at(i) * kRows + m_row]);
+    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
     const float ref = top == -kInf ? 0.0f : top;
-    float acc[DP / 32];
-#pragma unroll
-    for (int x = 0; x < DP / 32; ++x) acc[x] = 0.0f;
     float sum = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      const float w = gr::fast_exp2((i0 == 0 ? mine : (i0 + lane < parts ? P.part_lse[at(i0 + lane)] : -kInf)) - ref);
-      const int n = min(32, parts - i0);
-      for (int i = 0; i < n; i += 4) {
-        float2 v[4][DP / 64];
+    float4 acc[DP / 16];
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
+    for (int x = 0; x < DP / 16; ++x) acc[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int kAhead = DP == 256 ? 1 : 2;
+    for (int i = 0; i < parts; i += kAhead) {
+      float4 v[kAhead][DP / 16];
+      float w[kAhead];
 #pragma unroll
-          for (int x = 0; x < DP / 64; ++x)
-            v[y][x] = i + y < n ? *reinterpret_cast<const float2*>(P.part_o + at(i0 + i + y) * DP + x * 64 + lane * 2)
-                                : make_float2(0.0f, 0.0f);
+      for (int y = 0; y < kAhead; ++y) {
+        const int j = min(i + y, parts - 1);
+        w[y] = i + y < parts ? P.part_lse[at(j) * kRows + m_row] : -kInf;
+        const float4* o = P.part_o + (at(j) * (DP / 4) + quarter) * kRows + m_row;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const float wy = __shfl_sync(0xFFFFFFFFu, w, i + y);   // 0 behind the last part
-          sum += i + y < n ? wy : 0.0f;
+        for (int x = 0; x < DP / 16; ++x) v[y][x] = o[x * 4 * kRows];
+      }
 #pragma unroll
-          for (int x = 0; x < DP / 64; ++x) {
-            acc[2 * x] += wy * v[y][x].x;
-            acc[2 * x + 1] += wy * v[y][x].y;
-          }
+      for (int y = 0; y < kAhead; ++y) {
+        if (i + y >= parts) break;
+        const float wy = gr::fast_exp2(w[y] - ref);
+        sum += wy;
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          acc[x].x += wy * v[y][x].x;
+          acc[x].y += wy * v[y][x].y;
+          acc[x].z += wy * v[y][x].z;
+          acc[x].w += wy * v[y][x].w;
         }
       }
     }
+    if (!live) continue;
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     const int64_t t = static_cast<int64_t>(h.tok0) + tok;
     const int head = h.kvh * P.group + g;
     unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + head * P.out_head) * 2;
 #pragma unroll
-    for (int x = 0; x < DP / 64; ++x) {
-      const int col = x * 64 + lane * 2;
+    for (int x = 0; x < DP / 16; ++x) {
+      const int col = x * 16 + quarter * 4;
       if (col < P.dim)
-        *reinterpret_cast<uint32_t*>(orow + col * 2) = pack16<kBf16>(acc[2 * x] * inv, acc[2 * x + 1] * inv);
+        *reinterpret_cast<uint2*>(orow + col * 2) =
+            make_uint2(pack16<kBf16>(acc[x].x * inv, acc[x].y * inv), pack16<kBf16>(acc[x].z * inv, acc[x].w * inv));
     }
-    if (lane == 0 && P.lse)
+    if (quarter == 0 && P.lse)
       P.lse[t * P.heads + head] =
           sum > 0.0f || sum != sum ? (ref + __log2f(sum)) * 0.6931471805599453f : -kInf;
   }
@@ -1188,9 +1206,9 @@ static int run(const Params& P, const Geometry& g, const CUtensorMap& mq, const 
   if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, P.pre != nullptr, P, mq, mk, mv) !=
       cudaSuccess)
     return GR_ERR_CUDA;
-  // two rows of a block per warp of the join
+  // a block's rows in one pass of the join
   const int64_t rows = static_cast<int64_t>(g.longest < S::NQ * g.tp ? g.longest : S::NQ * g.tp) * g.group;
-  const int slices = static_cast<int>((rows + 2 * kJoinWarps - 1) / (2 * kJoinWarps));
+  const int slices = static_cast<int>((rows + kJoinRows - 1) / kJoinRows);
   if (ctas > 1 && launch(join_kernel<S::DP, S::NQ, kBf16>, dim3(ctas - 1, slices), kJoinThreads, 0, s, true, P,
                          ctas) != cudaSuccess)
     return GR_ERR_CUDA;
@@ -1270,13 +1288,15 @@ extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_page
   P.causal = d->causal;
   P.tp = g.tp;
   P.box = g.box;
+  P.out32 = (reinterpret_cast<uintptr_t>(io->out) & 31u) == 0 && d->head_dim % 16 == 0 &&
+            (d->out_stride_tok % 16 == 0 || d->num_tokens == 1) && (d->out_stride_head % 16 == 0 || d->num_heads == 1);
   const char* stall = std::getenv("GR_TEST_STALL_COPIES");
   P.flags = stall && stall[0] == '1' ? 1 : 0;
   P.scale = d->scale;
   P.scale_log2 = d->scale * gr::kLog2e;
   P.hdr = reinterpret_cast<Hdr*>(ws + l.hdr);
   P.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
-  P.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  P.part_o = reinterpret_cast<float4*>(ws + l.part_o);
   P.pre = nullptr;
   P.item = nullptr;
   P.num_items = nullptr;
