@@ -735,6 +735,11 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
   }
 }
 
+// The n lowest bits (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u);
+}
+
 // Warps 4..: softmax of one query tile, one thread per row; also the rare
 // rescaling of the accumulator, and the block's output.
 template <class S, bool kBf16>
@@ -782,11 +787,14 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
         tc_wait_ld();
         const bool whole = key0 + BN <= lim && (key0 + BN <= first || key0 >= own);
         if (!__all_sync(0xFFFFFFFFu, whole)) {
-          const int nl = lim - key0, nf = first - key0, no = own - key0;
+          // one bit per key, then one select per score (comparisons per score
+          // made this path 5 us per tile)
 #pragma unroll
-          for (int x = 0; x < BN; ++x) {
-            const bool see = x < nl && (x < nf || x >= no);
-            if (!see) sr[x / 32][x % 32] = 0xFF800000u;
+          for (int x = 0; x < BN / 32; ++x) {
+            const uint32_t see = low_bits(lim - key0 - x * 32) &
+                                 (low_bits(first - key0 - x * 32) | ~low_bits(own - key0 - x * 32));
+#pragma unroll
+            for (int y = 0; y < 32; ++y) sr[x][y] = see & (1u << y) ? sr[x][y] : 0xFF800000u;
           }
         }
         float t0 = -kInf, t1 = -kInf, t2 = -kInf, t3 = -kInf;
@@ -875,40 +883,51 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
       }
       unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
       float4* prt = P.part_o + (static_cast<int64_t>(part) * S::NQ + slot) * (DP / 4) * kRows + m_row;
+      constexpr int kCols = DP < 128 ? DP : 128;   // columns in registers at a time
 #pragma unroll 1
-      for (int x = 0; x < DP; x += 32) {
-        uint32_t o[32];
-        tc_ld32(o, o_col + x);
+      for (int x0 = 0; x0 < DP; x0 += kCols) {
+        uint32_t o[kCols / 32][32];
+#pragma unroll
+        for (int x = 0; x < kCols / 32; ++x) tc_ld32(o[x], o_col + x0 + x * 32);
         tc_wait_ld();
-        if (live) {
+        if (x0 + kCols >= DP) {   // read out: the next pair's products may begin
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->o_free[slot]);
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int x = 0; x < kCols / 32; ++x) {
           if (whole) {
 #pragma unroll
             for (int y = 0; y < 32; y += 16) {
               uint32_t v[8];
 #pragma unroll
               for (int z = 0; z < 8; ++z)
-                v[z] = pack16<kBf16>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
-              unsigned char* to = orow + (x + y) * 2;
+                v[z] = pack16<kBf16>(__uint_as_float(o[x][y + 2 * z]) * inv, __uint_as_float(o[x][y + 2 * z + 1]) * inv);
+              const int col = x0 + x * 32 + y;
+              unsigned char* to = orow + col * 2;
               if (P.out32) {            // whole sectors; the head dim is a multiple of 16 then
-                if (x + y < P.dim) st_global_32(to, v);
+                if (col < P.dim) st_global_32(to, v);
               } else {
-                if (x + y < P.dim) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-                if (x + y + 8 < P.dim) *reinterpret_cast<uint4*>(to + 16) = make_uint4(v[4], v[5], v[6], v[7]);
+                if (col < P.dim) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+                if (col + 8 < P.dim) *reinterpret_cast<uint4*>(to + 16) = make_uint4(v[4], v[5], v[6], v[7]);
               }
             }
           } else {
 #pragma unroll
             for (int y = 0; y < 32; y += 4)
-              prt[(x + y) / 4 * kRows] =
-                  make_float4(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv,
-                              __uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
+              prt[(x0 + x * 32 + y) / 4 * kRows] =
+                  make_float4(__uint_as_float(o[x][y]) * inv, __uint_as_float(o[x][y + 1]) * inv,
+                              __uint_as_float(o[x][y + 2]) * inv, __uint_as_float(o[x][y + 3]) * inv);
           }
         }
       }
+    } else {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->o_free[slot]);
     }
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh->o_free[slot]);
   }
 }
 
