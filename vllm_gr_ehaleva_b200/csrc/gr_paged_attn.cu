@@ -241,6 +241,12 @@ __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity)
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
 }
+// The same by one thread alone.
+__device__ __forceinline__ bool wait_one(Shared* sh, uint64_t* bar, uint32_t parity) {
+  if (gr::mbar_wait_bounded(bar, parity, &sh->abort)) return true;
+  *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+  return false;
+}
 
 // ---------------------------------------------------------------- geometry
 struct Seq {          // a request
@@ -598,24 +604,11 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
   }
 }
 
-// Value rows behind the last key hold whatever the block held before, and
-// 0 * NaN is NaN: they are zeroed before the product reads them.
-template <class S>
-__device__ __forceinline__ void zero_tail(uint32_t tile, int from, int to) {
-  const int lane = threadIdx.x & 31;
-  for (int e = lane; e < (to - from) * 8 * S::CH; e += 32) {
-    const int c = e / ((to - from) * 8), x = e - c * (to - from) * 8;
-    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * S::kChunkKV + from * 128 + x * 16), "r"(0)
-                 : "memory");
-  }
-  gr::fence_proxy_async_smem();
-  __syncwarp();
-}
-
-// Warp 1: the matrix products, issued by one lane.
+// Warp 1, one lane: the matrix products.  The issue of a product holds the thread
+// about as long as the product takes, so whatever the thread does between two
+// batches is time that the tensor pipe stands still: no votes, no warp-wide waits.
 template <class S, bool kBf16>
 __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t data) {
-  const int lane = threadIdx.x & 31;
   const uint32_t tmem = sh->tmem;
   const uint32_t ringbase = data + S::NQ * S::kQTile;
   constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
@@ -625,81 +618,74 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
       (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((S::DP / 8) << 17) | ((kRows / 16) << 24);
 
   const auto qk = [&](int q, int buf, int stage) {   // S[buf] = Q[q] K^T
-    if (lane == 0) {
-      const uint32_t qa = data + q * S::kQTile, ka = ringbase + stage * S::kStage;
+    const uint64_t qa = smem_desc(data + q * S::kQTile, 16, 1024);
+    const uint64_t ka = smem_desc(ringbase + stage * S::kStage, 16, 1024);
 #pragma unroll
-      for (int c = 0; c < S::CH; ++c)
+    for (int c = 0; c < S::CH; ++c)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          tc_mma_ss(tmem + buf * S::BN, smem_desc(qa + c * S::kChunkQ + x * 32, 16, 1024),
-                    smem_desc(ka + c * S::kChunkKV + x * 32, 16, 1024), kIdescS, (c | x) != 0);
-      tc_commit(&sh->s_full[buf]);
-    }
-    __syncwarp();
+      for (int x = 0; x < 4; ++x)
+        tc_mma_ss(tmem + buf * S::BN, qa + ((c * S::kChunkQ + x * 32) >> 4), ka + ((c * S::kChunkKV + x * 32) >> 4),
+                  kIdescS, (c | x) != 0);
+    tc_commit(&sh->s_full[buf]);
   };
   const auto pv = [&](int q, int buf, int stage, bool first) {   // O[q] (+)= P[buf] V
-    if (lane == 0) {
-      const uint32_t va = ringbase + stage * S::kStage;
+    const uint64_t va = smem_desc(ringbase + stage * S::kStage, S::kChunkKV, 1024);
 #pragma unroll
-      for (int x = 0; x < S::BN / 16; ++x)
-        tc_mma_ts(tmem + S::kColO + q * S::DP, tmem + buf * S::BN + x * 8,
-                  smem_desc(va + x * 2048, S::kChunkKV, 1024), kIdescO, !(first && x == 0));
-      tc_commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
-    }
-    __syncwarp();
-  };
-  const auto commit = [&](uint64_t* bar) {
-    if (lane == 0) tc_commit(bar);
-    __syncwarp();
+    for (int x = 0; x < S::BN / 16; ++x)
+      tc_mma_ts(tmem + S::kColO + q * S::DP, tmem + buf * S::BN + x * 8, va + ((x * 2048) >> 4), kIdescO,
+                !(first && x == 0));
+    tc_commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
   };
 
-  Work k;
   Ring<S> ring;
-  uint32_t seq = 0, qphase = 0, pphase = 0, ofree = 3;   // one bit per buffer / tile
+  uint32_t qphase = 0, pphase = 0, ofree = 3;   // one bit per buffer / tile
   uint32_t step = 0;    // score buffer of the next step (kNQ = 1)
-  while (next_work(sh, seq, k)) {
-    const int n = k.j1 - k.j0;
-    if (!wait(sh, &sh->q_full, qphase)) return;
+  const auto take = [&](int& stage) {           // the next key or value tile
+    if (!wait_one(sh, &sh->full[ring.stage], ring.phase)) return false;
+    tc_fence_after();
+    stage = ring.stage;
+    ring.next();
+    return true;
+  };
+  const auto probs = [&](int buf) {
+    if (!wait_one(sh, &sh->p_full[buf], (pphase >> buf) & 1u)) return false;
+    pphase ^= 1u << buf;
+    return true;
+  };
+  const auto o_free = [&](int q) {              // the accumulator's last contents are read
+    if (!wait_one(sh, &sh->o_free[q], (ofree >> q) & 1u)) return false;
+    ofree ^= 1u << q;
+    return true;
+  };
+  for (uint32_t seq = 0;; ++seq) {
+    const int at = seq % kWorkRing;
+    if (!wait_one(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u)) return;
+    const int slots = sh->work[at].slots, n = sh->work[at].j1 - sh->work[at].j0;
+    mbar_arrive(&sh->wk_empty[at]);
+    if (slots == 0) return;
+    if (!wait_one(sh, &sh->q_full, qphase)) return;
     qphase ^= 1u;
-    int kstage = 0;
-    const auto take = [&](int& stage) {
-      if (!wait(sh, &sh->full[ring.stage], ring.phase)) return false;
-      tc_fence_after();
-      stage = ring.stage;
-      ring.next();
-      return true;
-    };
-    const auto take_v = [&](int& stage, int j) {
-      if (!take(stage)) return false;
-      const int live = k.len - tile_at(k, k.j0 + j) * S::BN;
-      if (live > 0 && live < S::BN && live % P.box != 0)
-        zero_tail<S>(ringbase + stage * S::kStage, live, (live / P.box + 1) * P.box);
-      return true;
-    };
+    int kstage = 0, vstage = 0;
     if (S::NQ == 2) {
       if (!take(kstage)) return;
-      for (int q = 0; q < k.slots; ++q) qk(q, q, kstage);
-      commit(&sh->empty[kstage]);
-      if (n == 1) commit(&sh->q_empty);
+      for (int q = 0; q < slots; ++q) qk(q, q, kstage);
+      tc_commit(&sh->empty[kstage]);
+      if (n == 1) tc_commit(&sh->q_empty);
       for (int j = 0; j < n; ++j) {
-        int vstage = 0;
-        for (int q = 0; q < k.slots; ++q) {
-          if (!wait(sh, &sh->p_full[q], (pphase >> q) & 1u)) return;
-          pphase ^= 1u << q;
-          if (q == 0 && !take_v(vstage, j)) return;
-          if (j == 0) {
-            if (!wait(sh, &sh->o_free[q], (ofree >> q) & 1u)) return;
-            ofree ^= 1u << q;
-          }
+        for (int q = 0; q < slots; ++q) {
+          const bool last = q == slots - 1;
+          if (q == 0 && !take(vstage)) return;
+          if (j == 0 && !o_free(q)) return;
+          if (!probs(q)) return;
           tc_fence_after();
           pv(q, q, vstage, j == 0);
-          if (q == k.slots - 1) commit(&sh->empty[vstage]);
+          if (last) tc_commit(&sh->empty[vstage]);
           if (j + 1 < n) {
             if (q == 0 && !take(kstage)) return;
             qk(q, q, kstage);
-            if (q == k.slots - 1) {
-              commit(&sh->empty[kstage]);
-              if (j + 2 == n) commit(&sh->q_empty);
+            if (last) {
+              tc_commit(&sh->empty[kstage]);
+              if (j + 2 == n) tc_commit(&sh->q_empty);
             }
           }
         }
@@ -708,31 +694,46 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
       for (int j = 0; j < 2 && j < n; ++j) {
         if (!take(kstage)) return;
         qk(0, (step + j) & 1, kstage);
-        commit(&sh->empty[kstage]);
-        if (j + 1 == n) commit(&sh->q_empty);
+        tc_commit(&sh->empty[kstage]);
+        if (j + 1 == n) tc_commit(&sh->q_empty);
       }
       for (int j = 0; j < n; ++j, ++step) {
         const int b = step & 1;
-        int vstage = 0;
-        if (!wait(sh, &sh->p_full[b], (pphase >> b) & 1u)) return;
-        pphase ^= 1u << b;
-        if (!take_v(vstage, j)) return;
-        if (j == 0) {
-          if (!wait(sh, &sh->o_free[0], ofree & 1u)) return;
-          ofree ^= 1u;
-        }
+        if (!take(vstage)) return;
+        if (j == 0 && !o_free(0)) return;
+        if (!probs(b)) return;
         tc_fence_after();
         pv(0, b, vstage, j == 0);
-        commit(&sh->empty[vstage]);
+        tc_commit(&sh->empty[vstage]);
         if (j + 2 < n) {
           if (!take(kstage)) return;
           qk(0, b, kstage);
-          commit(&sh->empty[kstage]);
-          if (j + 3 == n) commit(&sh->q_empty);
+          tc_commit(&sh->empty[kstage]);
+          if (j + 3 == n) tc_commit(&sh->q_empty);
         }
       }
     }
   }
+}
+
+// Value rows behind the last key hold whatever the block held before, and
+// 0 * NaN is NaN: the softmax warps of the first tile zero them before they
+// hand over the probabilities that the product takes with these rows.
+template <class S>
+__device__ __forceinline__ void zero_tail(uint32_t tile, int from, int to) {
+  const int n = (to - from) * 8;
+  for (int e = threadIdx.x & 127; e < n * S::CH; e += 128) {
+    const int c = e / n, x = e - c * n;
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * S::kChunkKV + from * 128 + x * 16), "r"(0)
+                 : "memory");
+  }
+  gr::fence_proxy_async_smem();
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // The n lowest bits (none for n <= 0, all for n >= 32).
@@ -743,7 +744,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
 // Warps 4..: softmax of one query tile, one thread per row; also the rare
 // rescaling of the accumulator, and the block's output.
 template <class S, bool kBf16>
-__device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int slot) {
+__device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32_t data, int slot) {
   constexpr int BN = S::BN, DP = S::DP;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
   const int m_row = warp * 32 + lane;
@@ -754,8 +755,8 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
   const int ti = m_row / P.group, g = m_row - ti * P.group;
   Work k;
   uint32_t seq = 0, sphase = 0, pvphase = 0;   // one bit per buffer
-  uint32_t step = 0;
-  while (next_work(sh, seq, k)) {
+  uint32_t step = 0, tiles = 0;                // score buffer of the next step, tiles through the ring
+  for (; next_work(sh, seq, k); tiles += 2 * (k.j1 - k.j0)) {
     if (S::NQ == 2 && slot >= k.slots) continue;
     const int n = k.j1 - k.j0;
     // this row: token, position, the keys it sees
@@ -797,15 +798,13 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
             for (int y = 0; y < 32; ++y) sr[x][y] = see & (1u << y) ? sr[x][y] : 0xFF800000u;
           }
         }
-        float t0 = -kInf, t1 = -kInf, t2 = -kInf, t3 = -kInf;
+        float t[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
-        for (int x = 0; x < BN; x += 4) {
-          t0 = fmaxf(t0, __uint_as_float(sr[x / 32][x % 32]));
-          t1 = fmaxf(t1, __uint_as_float(sr[x / 32][x % 32 + 1]));
-          t2 = fmaxf(t2, __uint_as_float(sr[x / 32][x % 32 + 2]));
-          t3 = fmaxf(t3, __uint_as_float(sr[x / 32][x % 32 + 3]));
-        }
-        const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+        for (int x = 0; x < BN; x += 8)
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            t[y] = max3(t[y], __uint_as_float(sr[x / 32][x % 32 + 2 * y]), __uint_as_float(sr[x / 32][x % 32 + 2 * y + 1]));
+        const float top = max3(fmaxf(t[0], t[1]), t[2], t[3]);
         // a reference of its own for the row's first keys, then only when the growth is large
         const bool grow = live && ((top - m) * c > kRescale || (m == -kInf && top > -kInf));
         if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -855,6 +854,15 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, int sl
         float x0, x1;
         gr::unpack2(a0, x0, x1);
         l += x0 + x1;
+      }
+      if (j == n - 1 && slot == 0) {
+        // the pair's last value tile is the last in the ring so far
+        const int rows = k.len - key0;
+        if (rows > 0 && rows < BN && rows % P.box != 0) {
+          const uint32_t pos = tiles + 2 * n - 1, stage = pos % S::kStages;
+          if (!wait(sh, &sh->full[stage], (pos / S::kStages) & 1u)) return;
+          zero_tail<S>(data + S::NQ * S::kQTile + stage * S::kStage, rows, (rows / P.box + 1) * P.box);
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -989,8 +997,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     } else if (warp != 1 && busy) {
       load_role<S>(P, sh, base, &mq, &mk, &mv, warp >> 1);
     } else if (warp == 1 && busy) {
-      mma_role<S, kBf16>(P, sh, base);
-      if (sh->abort) {   // products in flight finish before the tensor memory goes
+      if (lane == 0) mma_role<S, kBf16>(P, sh, base);
+      __syncwarp();
+      if (*reinterpret_cast<volatile int*>(&sh->abort)) {   // products in flight finish before the tensor memory goes
         if (lane == 0) tc_commit(&sh->drain);
         __syncwarp();
         gr::mbar_wait_bounded(&sh->drain, 0);
@@ -998,7 +1007,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     }
   } else {
     if constexpr (S::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    if (busy) softmax_role<S, kBf16>(P, sh, (warp >> 2) - 1);
+    if (busy) softmax_role<S, kBf16>(P, sh, base, (warp >> 2) - 1);
   }
   __syncwarp();
   tc_fence_before();
