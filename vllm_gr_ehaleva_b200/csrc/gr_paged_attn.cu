@@ -25,8 +25,8 @@
 // ahead.  For beams, key tiles between the tail and the block's first beam hold
 // only other beams' tokens and are not visited.
 //
-// Kernel.  Warps 0 and 2 load (tensor-map copies of the blocks' rows, 128-byte
-// swizzle, a ring of key and value tiles), warp 1 issues the matrix products
+// Kernel.  Warps 0 and 2 load keys and values (tensor-map copies of the blocks'
+// rows, 128-byte swizzle, one ring of tiles), warp 1 issues the matrix products
 // (S = Q K^T from shared memory, O += P V with P in tensor memory), warp 3 walks
 // the run and hands out its (block, head) pairs; warps 4.. are the softmax: one thread per
 // row.  Two query tiles (kNQ = 2) have a softmax group each and alternate on the
@@ -130,6 +130,7 @@ struct Params {
   int block_size, max_blocks, causal;
   int tp;                          // query tokens per tile
   int box;                         // rows of a block that one copy takes
+  uint32_t div_mul, div_shift;     // x / block_size = (x * div_mul >> 32) >> div_shift for x < 2^31
   int out32;                       // output rows start on 32 bytes
   int flags;                       // 1: copies are not issued (test hook)
   float scale_log2, scale;
@@ -520,34 +521,27 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh, int c
   }
 }
 
-// Warps 0 and 2: the block's queries once (warp 0), then its key and value tiles
-// in the order in which the matrix products first use them, half of a tile's
-// copies each (blocks of 16 rows make 32 copies of a key and a value tile: one
-// warp cannot issue them at the rate of the memory).
-template <class S>
+// Warp 0: the block's queries once, then its key tiles; warp 2: its value tiles.
+// Tiles take the ring's stages in the order in which the products first use them:
+// K0 .. K(lead-1), V0, K(lead), V1, ...  A lane looks up one copy's block a tile
+// ahead, one lane issues the copies (lanes issuing their own took 100 cycles a
+// copy, and blocks of 16 rows make 32 copies of a key and a value tile).
+template <class S, bool kKeys>
 __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t data, const CUtensorMap* mq,
-                                          const CUtensorMap* mk, const CUtensorMap* mv, int half) {
+                                          const CUtensorMap* map) {
   const int lane = threadIdx.x & 31;
   Work k;
   Ring<S> ring;
-  uint32_t qphase = 0, seq = 0;
-  int64_t issued = 0;
+  uint32_t qphase = 0, seq = 0, mine = 0;       // mine: bit per stage this warp has filled
   bool q_issued = false, ok = true;
   const uint32_t ringbase = data + S::NQ * S::kQTile;
   const int boxes = S::BN / P.box;
-  // this lane's copy of a tile: column chunk c of box bx
-  const int per = (boxes * S::CH + 1) / 2;
-  const int e = half * per + lane, bx = e / S::CH, c = e - bx * S::CH;
-  const bool mine = lane < per && bx < boxes;
-  const uint32_t at = c * S::kChunkKV + bx * P.box * 128;
   const int oob = static_cast<int>(P.num_blocks);
+  constexpr int kLead = S::NQ == 2 ? 1 : 2;
   int bad = 0;
   while (ok && next_work(sh, seq, k)) {
-    if (half == 0) {
-      if (!wait(sh, &sh->q_empty, qphase ^ 1u)) {
-        ok = false;
-        break;
-      }
+    if (kKeys) {
+      if (!wait(sh, &sh->q_empty, qphase ^ 1u)) break;
       if (lane == 0 && !(P.flags & 1)) {
         const int slots = S::NQ == 2 ? k.slots : 1;
         mbar_arrive_expect_tx(&sh->q_full, static_cast<uint32_t>(slots * S::CH * P.group * P.tp * 128));
@@ -560,45 +554,55 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
       qphase ^= 1u;
     }
     const int n = k.j1 - k.j0;
-    const int lead = S::NQ == 2 ? 1 : 2;
     const int32_t* row = P.table + k.req * P.table_stride;
-    // the order K0 .. K(lead-1), V0, K(lead), V1, ...
-    for (int x = 0, ki = 0, vi = 0; x < 2 * n; ++x) {
-      const bool is_k = ki < n && ki < vi + lead;
-      const int j = is_k ? ki++ : vi++;
-      // the block id first, so that its latency overlaps the wait
-      const int tok = tile_at(k, k.j0 + j) * S::BN + bx * P.box;
-      int id = oob;
-      if (mine && tok < k.len) {
-        const int v = __ldg(row + tok / P.block_size);
+    // box `lane` of tile j: its block, and its first row in the block
+    const auto look = [&](int j, int& id, int& off) {
+      const int tok = tile_at(k, k.j0 + j) * S::BN + lane * P.box;
+      const int blk = static_cast<int>(__umulhi(static_cast<uint32_t>(tok), P.div_mul) >> P.div_shift);
+      id = oob;
+      off = tok - blk * P.block_size;
+      if (lane < boxes && tok < k.len) {
+        const int v = __ldg(row + blk);
         if (v < 0 || v >= oob) bad = 1; else id = v;
       }
+    };
+    int id, off;
+    look(0, id, off);
+    for (int x = 0, ki = 0, vi = 0; x < 2 * n; ++x, ring.next()) {
+      const bool is_k = ki < n && ki < vi + kLead;
+      const int j = is_k ? ki++ : vi++;
+      if (is_k != kKeys) continue;
+      const int id0 = id, off0 = off;
+      if (j + 1 < n) look(j + 1, id, off);
       if (!wait(sh, &sh->empty[ring.stage], ring.phase ^ 1u)) {
         ok = false;
         break;
       }
       if (!(P.flags & 1)) {
-        if (half == 0 && lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
-        __syncwarp();
-        if (mine)
-          tma_load4(ringbase + ring.stage * S::kStage + at, is_k ? mk : mv, c * 64, k.kvh, tok % P.block_size, id,
-                    &sh->full[ring.stage]);
-        ++issued;
+        if (lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
+        mine |= 1u << ring.stage;
+        const uint32_t dst = ringbase + ring.stage * S::kStage;
+        for (int i = 0; i < boxes; ++i) {
+          const int b = __shfl_sync(0xFFFFFFFFu, id0, i), r = __shfl_sync(0xFFFFFFFFu, off0, i);
+          if (lane == 0) {
+#pragma unroll
+            for (int c = 0; c < S::CH; ++c)
+              tma_load4(dst + c * S::kChunkKV + i * P.box * 128, map, c * 64, k.kvh, r, b, &sh->full[ring.stage]);
+          }
+        }
       }
-      ring.next();
     }
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_SLOT);
   if (*reinterpret_cast<volatile int*>(&sh->abort)) {
-    // gave up: wait (bounded) for the copies in flight before the shared memory goes
-    int64_t left = issued < S::kStages ? issued : S::kStages;
-    for (; left > 0; --left) {
+    // gave up: wait (bounded) for this warp's copies in flight before the shared memory goes
+    for (int i = 0; i < S::kStages; ++i) {
       if (ring.stage == 0) {
         ring.stage = S::kStages;
         ring.phase ^= 1u;
       }
       --ring.stage;
-      gr::mbar_wait_bounded(&sh->full[ring.stage], ring.phase);
+      if (mine >> ring.stage & 1u) gr::mbar_wait_bounded(&sh->full[ring.stage], ring.phase);
     }
     if (__any_sync(0xFFFFFFFFu, q_issued)) gr::mbar_wait_bounded(&sh->q_full, qphase ^ 1u);
   }
@@ -994,8 +998,10 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     if constexpr (S::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 3) {
       schedule_role<S>(P, sh, ctas);
-    } else if (warp != 1 && busy) {
-      load_role<S>(P, sh, base, &mq, &mk, &mv, warp >> 1);
+    } else if (warp == 0 && busy) {
+      load_role<S, true>(P, sh, base, &mq, &mk);
+    } else if (warp == 2 && busy) {
+      load_role<S, false>(P, sh, base, &mq, &mv);
     } else if (warp == 1 && busy) {
       if (lane == 0) mma_role<S, kBf16>(P, sh, base);
       __syncwarp();
@@ -1316,6 +1322,11 @@ extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_page
   P.causal = d->causal;
   P.tp = g.tp;
   P.box = g.box;
+  // x / d = x * m >> (32 + s) for every x < 2^31, with s = ceil(log2 d) - 1 and m = ceil(2^(32 + s) / d) < 2^32:
+  // x m = x 2^(32+s) / d + x e / d with e < d, and x e / d < 2^31 <= 2^(32+s) / d
+  P.div_shift = 0;
+  while ((2ll << P.div_shift) < d->block_size) ++P.div_shift;
+  P.div_mul = static_cast<uint32_t>(((1ull << (32 + P.div_shift)) + d->block_size - 1) / d->block_size);
   P.out32 = (reinterpret_cast<uintptr_t>(io->out) & 31u) == 0 && d->head_dim % 16 == 0 &&
             (d->out_stride_tok % 16 == 0 || d->num_tokens == 1) && (d->out_stride_head % 16 == 0 || d->num_heads == 1);
   const char* stall = std::getenv("GR_TEST_STALL_COPIES");
