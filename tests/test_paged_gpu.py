@@ -177,9 +177,8 @@ def test_long_caches_split_over_the_grid():
     b.check(*b.run(max_new=100))
 
 
-@pytest.mark.parametrize("R", [96, 97, 128, 700])
+@pytest.mark.parametrize("R", [97, 1024, 1025, 2300])
 def test_many_requests(R):
-    # up to 96 query blocks every CTA plans for itself, more go through the plan kernel
     rng = np.random.default_rng(R)
     ctx, new = rng.integers(0, 90, R), rng.integers(0, 3, R)
     b = Batch(ctx, new, 4, 2, 64, 16, BF16, seed=R)
@@ -187,8 +186,11 @@ def test_many_requests(R):
     b.check(*b.run(max_new=1000))           # a bound far above the longest query: the two-tile kernel
 
 
-def test_more_query_blocks_than_a_cta_plans():
+def test_many_query_blocks():
+    # more than one pass of the plan, and sums beyond its shared memory
     b = Batch([0, 17], [4500, 4000], 4, 1, 64, 16, F16, seed=17)
+    b.check(*b.run())
+    b = Batch([0] * 30, [90] * 30, 128, 1, 8, 8, BF16, seed=18)
     b.check(*b.run())
 
 

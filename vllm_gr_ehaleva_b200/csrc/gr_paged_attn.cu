@@ -16,14 +16,16 @@
 // Single tokens use group rows of the 128; their product time hides behind the
 // cache reads, which bound them.
 //
-// Work.  A (query block, KV head) of n key tiles costs n + kCost units; the
+// Work.  A (query block, KV head) pair of n key tiles costs n + kCost units; the
 // batch's units, in order, are cut into equal runs, one per CTA (one persistent
-// CTA per SM), whatever the lengths.  A (block, head) cut by a run's end leaves
-// partial outputs and log-sums in the workspace, joined by a second, small
-// kernel in a fixed order.  The prefix sums of the units come from a plan: up to
-// 96 query blocks are planned by every CTA for itself, more by a one-CTA kernel
-// ahead.  For beams, key tiles between the tail and the block's first beam hold
-// only other beams' tokens and are not visited.
+// CTA per SM), whatever the lengths (plan_kernel, one CTA, ahead).  A border that
+// falls into a short pair moves to the pair's nearer end; a longer pair is cut.
+// The CTA with a cut pair's end owns it: the others leave partial outputs and
+// log-sums in the workspace, which the owner joins in run order.  CTAs walk their
+// runs from the end, so that an owner comes to the join last and the parts that
+// it waits for came first in theirs, and it waits for lower-numbered CTAs only,
+// which never wait for it.  For beams, key tiles between the tail and the block's
+// first beam hold only other beams' tokens and are not visited.
 //
 // Kernel.  Warps 0 and 2 load keys and values (tensor-map copies of the blocks'
 // rows, 128-byte swizzle, one ring of tiles), warp 1 issues the matrix products
@@ -55,12 +57,19 @@ using gr::smem_u32;
 
 constexpr int kRows = 128;            // rows of a query tile (the matrix product's M)
 constexpr int kMaxCtas = 160;
-constexpr int kSmemPlan = 96;         // query blocks that a CTA plans for itself
 constexpr int kWorkRing = 4;          // (block, head) pairs handed out ahead
 #ifndef GR_PA_COST
 #define GR_PA_COST 2
 #endif
-constexpr int kCost = GR_PA_COST;     // what a (block, head) costs besides its key tiles, in key tiles
+constexpr int kCost = GR_PA_COST;     // what a pair costs besides its key tiles, in key tiles
+#ifndef GR_PA_SNAP
+#define GR_PA_SNAP 8
+#endif
+constexpr int kSnap = GR_PA_SNAP;     // longest pair, in units, that is never cut
+#ifndef GR_PA_MINRUN
+#define GR_PA_MINRUN 2
+#endif
+constexpr int kMinRun = GR_PA_MINRUN; // units that a CTA's run has at least, on average
 constexpr int kSmemMax = 232448;      // shared memory a CTA may have
 constexpr float kRescale = 8.0f;      // log2 of the growth of the maximum that is let stand
 
@@ -91,7 +100,7 @@ struct Work {
   int ta, tb, n;           // its key tiles: [0, ta) and from tb on, n in all
   int j0, j1;              // those of the run
   int slots;               // query tiles with rows; 0: the run is over
-  int pad;
+  int part0;               // the first CTA with a part of the pair (this one's pair: j0 > 0, j1 = n)
 };
 
 struct Shared {
@@ -102,18 +111,13 @@ struct Shared {
   uint64_t s_full[2], p_full[2];   // scores ready / probabilities ready
   uint64_t pv_done[2], o_free[2];  // product into O finished / O read out
   uint64_t drain;
-  int64_t pre[kSmemPlan + 1];
-  int32_t item[kSmemPlan];         // request | block << 8
-  int32_t num_items;
   uint32_t tmem;
   int abort;
 };
 
-struct Hdr {                       // a CTA's run, for the join
-  int64_t u0;                      // where it starts, in cost units
-  int64_t beg, end;                // cost range of the (block, head) it starts in
-  int32_t tok0, ntok;              // that block's query tokens
-  int32_t kvh, mid;                // its KV head; whether the run starts inside its key tiles
+struct Run {                       // where a CTA's run starts
+  int64_t u;                       // in units of the batch
+  int32_t item, pad;               // the query block that the run before it ends in
 };
 
 struct Params {
@@ -135,12 +139,12 @@ struct Params {
   int flags;                       // 1: copies are not issued (test hook)
   float scale_log2, scale;
   // plan and partials in the workspace
-  int64_t* pre;                    // [items + 1]; NULL: planned in shared memory
+  int64_t* pre;                    // [items + 1] units before each query block
   int2* item;                      // request, block
-  int32_t* num_items;
-  Hdr* hdr;
+  Run* run;                        // [ctas + 1]
+  int32_t* flag;                   // [ctas][2][4] part written (query tile, warp of it)
   float4* part_o;                  // [ctas][2][NQ][DP / 4][128 rows]: a warp's stores of its 32 rows are whole lines
-  float* part_lse;                 // [ctas][2][NQ * 128]
+  float* part_lse;                 // [ctas][2][NQ][128 rows]
 };
 
 // ---------------------------------------------------------------- tensor core
@@ -242,13 +246,6 @@ __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity)
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
 }
-// The same by one thread alone.
-__device__ __forceinline__ bool wait_one(Shared* sh, uint64_t* bar, uint32_t parity) {
-  if (gr::mbar_wait_bounded(bar, parity, &sh->abort)) return true;
-  *reinterpret_cast<volatile int*>(&sh->abort) = 1;
-  return false;
-}
-
 // ---------------------------------------------------------------- geometry
 struct Seq {          // a request
   int q0, n, len;     // first query token, query tokens, keys
@@ -309,43 +306,6 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
   return v;
 }
 
-// The plan of a small batch (at most kSmemPlan requests and query blocks, as the
-// host has bounded them), by one warp into shared memory.
-template <class S>
-__device__ void plan_warp(const Params& P, Shared* sh) {
-  const int lane = threadIdx.x & 31;
-  const int per = S::NQ * P.tp;
-  int64_t items = 0;
-  for (int r0 = 0; r0 < P.num_seqs; r0 += 32) {
-    const int r = r0 + lane;
-    int nb = 0;
-    if (r < P.num_seqs) nb = blocks_of(load_seq(P, r), per);
-    const int64_t inc = warp_scan(nb);
-    const int64_t first = items + inc - nb;
-    for (int b = 0; b < nb && first + b < kSmemPlan; ++b) sh->item[first + b] = r | (b << 8);
-    items += __shfl_sync(0xFFFFFFFFu, inc, 31);
-  }
-  if (items > kSmemPlan) items = kSmemPlan;
-  __syncwarp();
-  int64_t units = 0;
-  for (int i0 = 0; i0 < items; i0 += 32) {
-    const int i = i0 + lane;
-    int64_t u = 0;
-    if (i < items) {
-      const int r = sh->item[i] & 255, b = sh->item[i] >> 8;
-      const Seq s = load_seq(P, r);
-      u = static_cast<int64_t>(key_tiles<S::BN>(s, P.causal, b * per, min(s.n, (b + 1) * per)).n + kCost) * P.kv_heads;
-    }
-    const int64_t inc = warp_scan(u);
-    if (i < items) sh->pre[i] = units + inc - u;
-    units += __shfl_sync(0xFFFFFFFFu, inc, 31);
-  }
-  if (lane == 0) {
-    sh->pre[items] = units;
-    sh->num_items = static_cast<int>(items);
-  }
-}
-
 constexpr int kPlanThreads = 1024;
 
 // Exclusive sum over a CTA of kPlanThreads; total in `total`.
@@ -366,20 +326,26 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t
   return part[warp] + inc - v;
 }
 
-// The plan of a larger batch, in the workspace: items (request, block) in order
-// and the exclusive sums of their units.
+// The plan, by one CTA: the query blocks (request, block) in order, the exclusive
+// sums of their units, and the borders of the CTAs' runs.
+constexpr int kPlanItems = 2048;   // sums kept in shared memory for the search of the borders
+
 template <int BN>
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int per, int max_items) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int per, int max_items, int ctas) {
   __shared__ int64_t part[33];
+  __shared__ int64_t s_pre[kPlanItems + 1];
   gr::pdl_trigger();
+  for (int i = threadIdx.x; i < ctas * 8; i += kPlanThreads) P.flag[i] = 0;
   int64_t items = 0, total;
+  int bad = 0;
   for (int r0 = 0; r0 < P.num_seqs; r0 += kPlanThreads) {
     const int r = r0 + static_cast<int>(threadIdx.x);
-    const int nb = r < P.num_seqs ? blocks_of(load_seq(P, r), per) : 0;
+    const int nb = r < P.num_seqs ? blocks_of(load_seq(P, r, &bad), per) : 0;
     const int64_t first = items + block_scan(nb, total, part);
     for (int b = 0; b < nb && first + b < max_items; ++b) P.item[first + b] = make_int2(r, b);
     items += total;
   }
+  if (bad && P.err) atomicOr(P.err, GR_DEVERR_BAD_RECORD);
   if (items > max_items) items = max_items;
   __syncthreads();
   int64_t units = 0;
@@ -392,12 +358,38 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
       u = static_cast<int64_t>(key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n + kCost) * P.kv_heads;
     }
     const int64_t ex = block_scan(u, total, part);
-    if (i < items) P.pre[i] = units + ex;
+    if (i < items) {
+      P.pre[i] = units + ex;
+      if (i < kPlanItems) s_pre[i] = units + ex;
+    }
     units += total;
   }
   if (threadIdx.x == 0) {
     P.pre[items] = units;
-    P.num_items[0] = static_cast<int>(items);
+    if (items <= kPlanItems) s_pre[items] = units;
+  }
+  __syncthreads();
+  // border c; runs behind the last one of use are empty
+  const int64_t* pre = items <= kPlanItems ? s_pre : P.pre;
+  const int64_t runs = items == 0 ? 0 : min(static_cast<int64_t>(ctas), max(units / kMinRun, static_cast<int64_t>(1)));
+  for (int c = threadIdx.x; c <= ctas; c += kPlanThreads) {
+    Run run{units, static_cast<int>(items) - 1, 0};
+    if (c < runs) {
+      int64_t u = units * c / runs;
+      int lo = 0, hi = static_cast<int>(items) - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] <= u) lo = mid; else hi = mid - 1;
+      }
+      const int span = static_cast<int>((pre[lo + 1] - pre[lo]) / P.kv_heads);
+      if (span <= kSnap) {
+        const int off = static_cast<int>((u - pre[lo]) % span);
+        u += 2 * off < span ? -off : span - off;
+      }
+      run.u = u;
+      run.item = u > pre[lo] ? lo : lo - 1;   // the block of unit u - 1
+    }
+    P.run[c] = run;
   }
 }
 
@@ -427,83 +419,53 @@ __device__ __forceinline__ bool next_work(Shared* sh, uint32_t& seq, Work& k) {
   return k.slots > 0;
 }
 
-// Warp 3: walks the CTA's run [cost * cta / ctas, cost * (cta + 1) / ctas) of the
-// batch's cost and hands out its (block, head) pairs ahead of their use.  A pair
-// of n key tiles spans kCost + n units: a border in the first kCost leaves it
-// whole, a border behind cuts its key tiles.  Also the header for the join.
+// Warp 3: walks the CTA's run from its end and hands out its pairs ahead of their
+// use.  A pair of n key tiles spans kCost + n units: a border in the first kCost
+// leaves it whole, a border behind cuts its key tiles.
 template <class S>
-__device__ __forceinline__ void schedule_role(const Params& P, Shared* sh, int ctas) {
+__device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
   const int lane = threadIdx.x & 31;
-  const int64_t* pre = P.pre ? P.pre : sh->pre;
-  const int items = P.pre ? P.num_items[0] : sh->num_items;
-  const int64_t units = pre[items];
-  Hdr h{units, 0, 0, 0, 0, 0, 0};
-  if (static_cast<int>(blockIdx.x) >= ctas) {
-    if (lane == 0) P.hdr[blockIdx.x] = h;
-    return;
-  }
-  int64_t u = units * blockIdx.x / ctas;
-  const int64_t end = units * (blockIdx.x + 1) / ctas;
-  h.u0 = u;
-  int lo = 0, hi = items - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= u) lo = mid; else hi = mid - 1;
-  }
+  const int64_t begin = P.run[blockIdx.x].u;
+  const Run stop = P.run[blockIdx.x + 1];
+  int64_t u = stop.u;
   const int per = S::NQ * P.tp;
-  bool first = true;
   uint32_t seq = 0;
-  for (int i = lo; u < end; ++i) {
-    int r, b;
-    if (P.pre) {
-      const int2 it = P.item[i];
-      r = it.x;
-      b = it.y;
-    } else {
-      r = sh->item[i] & 255;
-      b = sh->item[i] >> 8;
-    }
-    const Seq s = load_seq(P, r);
+  for (int i = stop.item; u > begin; --i) {
+    const int2 it = P.item[i];
+    const Seq s = load_seq(P, it.x);
     Work k;
-    k.req = r;
+    k.req = it.x;
     k.q0 = s.q0;
     k.len = s.len;
     k.ctx = s.ctx;
     k.tail = s.tail;
     k.steps = s.steps;
-    k.t0 = b * per;
+    k.t0 = it.y * per;
     k.nt = min(s.n - k.t0, per);
     k.slots = k.nt > P.tp ? 2 : 1;
-    k.pad = 0;
     const Tiles t = key_tiles<S::BN>(s, P.causal, k.t0, k.t0 + k.nt);
     k.ta = t.a;
     k.tb = t.b;
     k.n = t.n;
     const int span = t.n + kCost;
-    const int64_t in = u - pre[i];
-    int off = 0;
-    k.kvh = 0;
-    if (in > 0) {
-      k.kvh = static_cast<int>(in / span);
-      off = static_cast<int>(in - static_cast<int64_t>(k.kvh) * span);
+    const int64_t base = P.pre[i];
+    k.kvh = P.kv_heads - 1;
+    int hi = span;                                   // end of the run in the pair
+    const int64_t in = u - base;
+    if (in < static_cast<int64_t>(span) * P.kv_heads) {
+      k.kvh = static_cast<int>((in - 1) / span);
+      hi = static_cast<int>(in - static_cast<int64_t>(k.kvh) * span);
     }
-    for (; k.kvh < P.kv_heads && u < end; ++k.kvh, off = 0) {
-      const int64_t beg = u - off;
-      const int stop = static_cast<int>(min(static_cast<int64_t>(span), off + (end - u)));
-      k.j0 = max(off - kCost, 0);
-      k.j1 = max(stop - kCost, 0);
-      u += stop - off;
-      if (first) {
-        first = false;
-        h.beg = beg;
-        h.end = beg + span;
-        h.tok0 = s.q0 + k.t0;
-        h.ntok = k.nt;
-        h.kvh = k.kvh;
-        h.mid = k.j0 > 0;
-        if (lane == 0) P.hdr[blockIdx.x] = h;
-      }
+    for (; k.kvh >= 0 && u > begin; --k.kvh, hi = span) {
+      const int64_t beg = u - hi;
+      const int lo = static_cast<int>(max(begin - beg, static_cast<int64_t>(0)));
+      k.j0 = max(lo - kCost, 0);
+      k.j1 = max(hi - kCost, 0);
+      u = beg + lo;
       if (k.j1 <= k.j0) continue;
+      k.part0 = blockIdx.x;
+      if (k.j0 > 0 && k.j1 == k.n)                   // this CTA joins the parts
+        do --k.part0; while (k.part0 > 0 && P.run[k.part0].u > beg + kCost);
       const int at = seq % kWorkRing;
       if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
       if (lane == 0) {
@@ -608,12 +570,19 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
   }
 }
 
-// Warp 1, one lane: the matrix products.  The issue of a product holds the thread
-// about as long as the product takes, so whatever the thread does between two
-// batches is time that the tensor pipe stands still: no votes, no warp-wide waits.
+// Warp 1: the matrix products, issued by one lane.  The issue of a product holds
+// the warp about as long as the product takes, so whatever it does between two
+// batches is time that the tensor pipe stands still.  All control flow is by the
+// whole warp, so that operands are known to be uniform (3 to 6 % fewer cycles than
+// a role of one lane, 2048-key prompts and beams).
 template <class S, bool kBf16>
 __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t data) {
-  const uint32_t tmem = sh->tmem;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, sh->tmem, 0);
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(leader));
+  const auto commit = [&](uint64_t* bar) {
+    if (leader) tc_commit(bar);
+  };
   const uint32_t ringbase = data + S::NQ * S::kQTile;
   constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
   // fp32 accumulators, A and B of one type, M = 128; B of the second product is stored along N
@@ -624,57 +593,62 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
   const auto qk = [&](int q, int buf, int stage) {   // S[buf] = Q[q] K^T
     const uint64_t qa = smem_desc(data + q * S::kQTile, 16, 1024);
     const uint64_t ka = smem_desc(ringbase + stage * S::kStage, 16, 1024);
+    if (leader) {
 #pragma unroll
-    for (int c = 0; c < S::CH; ++c)
+      for (int c = 0; c < S::CH; ++c)
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        tc_mma_ss(tmem + buf * S::BN, qa + ((c * S::kChunkQ + x * 32) >> 4), ka + ((c * S::kChunkKV + x * 32) >> 4),
-                  kIdescS, (c | x) != 0);
-    tc_commit(&sh->s_full[buf]);
+        for (int x = 0; x < 4; ++x)
+          tc_mma_ss(tmem + buf * S::BN, qa + ((c * S::kChunkQ + x * 32) >> 4), ka + ((c * S::kChunkKV + x * 32) >> 4),
+                    kIdescS, (c | x) != 0);
+    }
+    commit(&sh->s_full[buf]);
   };
   const auto pv = [&](int q, int buf, int stage, bool first) {   // O[q] (+)= P[buf] V
     const uint64_t va = smem_desc(ringbase + stage * S::kStage, S::kChunkKV, 1024);
+    if (leader) {
 #pragma unroll
-    for (int x = 0; x < S::BN / 16; ++x)
-      tc_mma_ts(tmem + S::kColO + q * S::DP, tmem + buf * S::BN + x * 8, va + ((x * 2048) >> 4), kIdescO,
-                !(first && x == 0));
-    tc_commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
+      for (int x = 0; x < S::BN / 16; ++x)
+        tc_mma_ts(tmem + S::kColO + q * S::DP, tmem + buf * S::BN + x * 8, va + ((x * 2048) >> 4), kIdescO,
+                  !(first && x == 0));
+    }
+    commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
   };
 
   Ring<S> ring;
   uint32_t qphase = 0, pphase = 0, ofree = 3;   // one bit per buffer / tile
   uint32_t step = 0;    // score buffer of the next step (kNQ = 1)
   const auto take = [&](int& stage) {           // the next key or value tile
-    if (!wait_one(sh, &sh->full[ring.stage], ring.phase)) return false;
+    if (!wait(sh, &sh->full[ring.stage], ring.phase)) return false;
     tc_fence_after();
     stage = ring.stage;
     ring.next();
     return true;
   };
   const auto probs = [&](int buf) {
-    if (!wait_one(sh, &sh->p_full[buf], (pphase >> buf) & 1u)) return false;
+    if (!wait(sh, &sh->p_full[buf], (pphase >> buf) & 1u)) return false;
     pphase ^= 1u << buf;
     return true;
   };
   const auto o_free = [&](int q) {              // the accumulator's last contents are read
-    if (!wait_one(sh, &sh->o_free[q], (ofree >> q) & 1u)) return false;
+    if (!wait(sh, &sh->o_free[q], (ofree >> q) & 1u)) return false;
     ofree ^= 1u << q;
     return true;
   };
   for (uint32_t seq = 0;; ++seq) {
     const int at = seq % kWorkRing;
-    if (!wait_one(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u)) return;
-    const int slots = sh->work[at].slots, n = sh->work[at].j1 - sh->work[at].j0;
-    mbar_arrive(&sh->wk_empty[at]);
+    if (!wait(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u)) return;
+    const int slots = __shfl_sync(0xFFFFFFFFu, sh->work[at].slots, 0);
+    const int n = __shfl_sync(0xFFFFFFFFu, sh->work[at].j1 - sh->work[at].j0, 0);
+    if (leader) mbar_arrive(&sh->wk_empty[at]);
     if (slots == 0) return;
-    if (!wait_one(sh, &sh->q_full, qphase)) return;
+    if (!wait(sh, &sh->q_full, qphase)) return;
     qphase ^= 1u;
     int kstage = 0, vstage = 0;
     if (S::NQ == 2) {
       if (!take(kstage)) return;
       for (int q = 0; q < slots; ++q) qk(q, q, kstage);
-      tc_commit(&sh->empty[kstage]);
-      if (n == 1) tc_commit(&sh->q_empty);
+      commit(&sh->empty[kstage]);
+      if (n == 1) commit(&sh->q_empty);
       for (int j = 0; j < n; ++j) {
         for (int q = 0; q < slots; ++q) {
           const bool last = q == slots - 1;
@@ -683,13 +657,13 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
           if (!probs(q)) return;
           tc_fence_after();
           pv(q, q, vstage, j == 0);
-          if (last) tc_commit(&sh->empty[vstage]);
+          if (last) commit(&sh->empty[vstage]);
           if (j + 1 < n) {
             if (q == 0 && !take(kstage)) return;
             qk(q, q, kstage);
             if (last) {
-              tc_commit(&sh->empty[kstage]);
-              if (j + 2 == n) tc_commit(&sh->q_empty);
+              commit(&sh->empty[kstage]);
+              if (j + 2 == n) commit(&sh->q_empty);
             }
           }
         }
@@ -698,8 +672,8 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
       for (int j = 0; j < 2 && j < n; ++j) {
         if (!take(kstage)) return;
         qk(0, (step + j) & 1, kstage);
-        tc_commit(&sh->empty[kstage]);
-        if (j + 1 == n) tc_commit(&sh->q_empty);
+        commit(&sh->empty[kstage]);
+        if (j + 1 == n) commit(&sh->q_empty);
       }
       for (int j = 0; j < n; ++j, ++step) {
         const int b = step & 1;
@@ -708,12 +682,12 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
         if (!probs(b)) return;
         tc_fence_after();
         pv(0, b, vstage, j == 0);
-        tc_commit(&sh->empty[vstage]);
+        commit(&sh->empty[vstage]);
         if (j + 2 < n) {
           if (!take(kstage)) return;
           qk(0, b, kstage);
-          tc_commit(&sh->empty[kstage]);
-          if (j + 3 == n) tc_commit(&sh->q_empty);
+          commit(&sh->empty[kstage]);
+          if (j + 3 == n) commit(&sh->q_empty);
         }
       }
     }
@@ -738,6 +712,118 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void st_release(int32_t* p, int32_t v) {
+  asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ int32_t ld_acquire(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// 32 output columns from col on, as far as the head dim goes.
+template <bool kBf16>
+__device__ __forceinline__ void store32(const Params& P, unsigned char* row, int col, const float4 (&v)[8]) {
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    uint32_t w[8];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      w[2 * z] = pack16<kBf16>(v[4 * y + z].x, v[4 * y + z].y);
+      w[2 * z + 1] = pack16<kBf16>(v[4 * y + z].z, v[4 * y + z].w);
+    }
+    const int at = col + y * 16;
+    unsigned char* to = row + at * 2;
+    if (P.out32) {            // whole sectors; the head dim is a multiple of 16 then
+      if (at < P.dim) st_global_32(to, w);
+    } else {
+      if (at < P.dim) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (at + 8 < P.dim) *reinterpret_cast<uint4*>(to + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+}
+
+// The rows of one warp of a cut pair, joined by the CTA that has the pair's end:
+// out = sum_i 2^(lse_i - top) out_i / sum_i 2^(lse_i - top) over the parts in run
+// order.  Few rows (single tokens cut over many CTAs) have two or four lanes each.
+template <class S, bool kBf16>
+__device__ __forceinline__ bool join(const Params& P, Shared* sh, const Work& k, int slot, int warp) {
+  constexpr int DP = S::DP;
+  const int lane = threadIdx.x & 31;
+  const int cta = blockIdx.x, parts = cta - k.part0 + 1;
+  // every part's flag (bounded), 32 at a time
+  bool ok = true;
+  const uint64_t since = gr::global_timer_ns();
+  for (int p = k.part0 + lane; p < cta; p += 32) {
+    while (ok && ld_acquire(P.flag + (p * 2 + slot) * 4 + warp) == 0)
+      ok = *reinterpret_cast<volatile int*>(&sh->abort) == 0 && gr::global_timer_ns() - since < gr::kWaitLimitNs;
+  }
+  if (!__all_sync(0xFFFFFFFFu, ok)) {
+    *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+    return false;
+  }
+  // the warp's rows: token rows are the first lanes'
+  const int rows = min(min(k.nt - slot * P.tp, P.tp) * P.group - warp * 32, 32);
+  const int each = rows <= 8 ? 4 : (rows <= 16 ? 2 : 1);   // lanes per row
+  const int r = lane % (32 / each), q = lane / (32 / each);
+  const int m_row = warp * 32 + min(r, rows - 1);
+  const auto place = [&](int i) {   // part i: the other CTAs' place 1, this one's place 0
+    const int p = k.part0 + i;
+    return (static_cast<int64_t>(p) * 2 + (p == cta ? 0 : 1)) * S::NQ + slot;
+  };
+  float top = -kInf;
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(P.part_lse + place(i) * kRows + m_row));
+  const float ref = top == -kInf ? 0.0f : top;
+  const int ti = m_row / P.group, g = m_row - ti * P.group;
+  const int64_t t = static_cast<int64_t>(k.q0) + k.t0 + slot * P.tp + ti;
+  const int h = k.kvh * P.group + g;
+  unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
+  constexpr int kAhead = 2;
+  for (int x = q * 32; x < DP; x += each * 32) {
+    float4 acc[8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) acc[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    for (int i = 0; i < parts; i += kAhead) {
+      float4 v[kAhead][8];
+      float w[kAhead];
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        if (i + z >= parts) break;
+        const int64_t at = place(i + z);
+        w[z] = __ldcg(P.part_lse + at * kRows + m_row);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) v[z][y] = __ldcg(P.part_o + (at * (DP / 4) + x / 4 + y) * kRows + m_row);
+      }
+#pragma unroll
+      for (int z = 0; z < kAhead; ++z) {
+        if (i + z >= parts) break;
+        const float wz = gr::fast_exp2(w[z] - ref);
+        sum += wz;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          acc[y].x += wz * v[z][y].x;
+          acc[y].y += wz * v[z][y].y;
+          acc[y].z += wz * v[z][y].z;
+          acc[y].w += wz * v[z][y].w;
+        }
+      }
+    }
+    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+      acc[y] = make_float4(acc[y].x * inv, acc[y].y * inv, acc[y].z * inv, acc[y].w * inv);
+    if (r < rows) {
+      store32<kBf16>(P, orow, x, acc);
+      if (x == 0 && P.lse)
+        P.lse[t * P.heads + h] = sum > 0.0f || sum != sum ? (ref + __log2f(sum)) * kLn2 : -kInf;
+    }
+  }
+  return true;
 }
 
 // The n lowest bits (none for n <= 0, all for n >= 32).
@@ -879,22 +965,24 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
     tc_fence_after();
     if (S::NQ == 1) step += n;
     const bool whole = k.j0 == 0 && k.j1 == k.n;
+    const bool owner = k.j0 > 0 && k.j1 == k.n;
+    // a cut pair's part goes to place 1 of this CTA, where its owner looks for it; the owner's
+    // own part to place 0
+    const int64_t place = (static_cast<int64_t>(blockIdx.x) * 2 + (owner ? 0 : 1)) * S::NQ + slot;
     if (any_live) {
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       const float lse2 = l > 0.0f || l != l ? m * c + __log2f(l) : -kInf;
       const int64_t t = static_cast<int64_t>(k.q0) + tok;
       const int h = k.kvh * P.group + g;
-      const int part = blockIdx.x * 2 + (k.j0 == 0 ? 1 : 0);
-      const int prow = slot * kRows + m_row;
       if (live) {
         if (whole) {
-          if (P.lse) P.lse[t * P.heads + h] = lse2 * 0.6931471805599453f;
+          if (P.lse) P.lse[t * P.heads + h] = lse2 * kLn2;
         } else {
-          P.part_lse[static_cast<int64_t>(part) * S::NQ * kRows + prow] = lse2;
+          P.part_lse[place * kRows + m_row] = lse2;
         }
       }
       unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
-      float4* prt = P.part_o + (static_cast<int64_t>(part) * S::NQ + slot) * (DP / 4) * kRows + m_row;
+      float4* prt = P.part_o + place * (DP / 4) * kRows + m_row;
       constexpr int kCols = DP < 128 ? DP : 128;   // columns in registers at a time
 #pragma unroll 1
       for (int x0 = 0; x0 < DP; x0 += kCols) {
@@ -911,21 +999,12 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
 #pragma unroll
         for (int x = 0; x < kCols / 32; ++x) {
           if (whole) {
+            float4 v[8];
 #pragma unroll
-            for (int y = 0; y < 32; y += 16) {
-              uint32_t v[8];
-#pragma unroll
-              for (int z = 0; z < 8; ++z)
-                v[z] = pack16<kBf16>(__uint_as_float(o[x][y + 2 * z]) * inv, __uint_as_float(o[x][y + 2 * z + 1]) * inv);
-              const int col = x0 + x * 32 + y;
-              unsigned char* to = orow + col * 2;
-              if (P.out32) {            // whole sectors; the head dim is a multiple of 16 then
-                if (col < P.dim) st_global_32(to, v);
-              } else {
-                if (col < P.dim) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-                if (col + 8 < P.dim) *reinterpret_cast<uint4*>(to + 16) = make_uint4(v[4], v[5], v[6], v[7]);
-              }
-            }
+            for (int y = 0; y < 8; ++y)
+              v[y] = make_float4(__uint_as_float(o[x][4 * y]) * inv, __uint_as_float(o[x][4 * y + 1]) * inv,
+                                 __uint_as_float(o[x][4 * y + 2]) * inv, __uint_as_float(o[x][4 * y + 3]) * inv);
+            store32<kBf16>(P, orow, x0 + x * 32, v);
           } else {
 #pragma unroll
             for (int y = 0; y < 32; y += 4)
@@ -933,6 +1012,15 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
                   make_float4(__uint_as_float(o[x][y]) * inv, __uint_as_float(o[x][y + 1]) * inv,
                               __uint_as_float(o[x][y + 2]) * inv, __uint_as_float(o[x][y + 3]) * inv);
           }
+        }
+      }
+      if (!whole) {
+        __threadfence();
+        __syncwarp();
+        if (!owner) {
+          if (lane == 0) st_release(P.flag + (blockIdx.x * 2 + slot) * 4 + warp, 1);
+        } else if (!join<S, kBf16>(P, sh, k, slot, warp)) {
+          return;
         }
       }
     } else {
@@ -977,34 +1065,23 @@ __global__ void __launch_bounds__(S::kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  gr::pdl_wait();      // the plan (or whatever came before) is complete
-  gr::pdl_trigger();
-  if (warp == 3 && P.pre == nullptr) plan_warp<S>(P, sh);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
 
-  // units per CTA: as many CTAs as there are units to share, at most the grid
-  const int64_t units = P.pre ? P.pre[P.num_items[0]] : sh->pre[sh->num_items];
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), units));
-  const bool busy = static_cast<int>(blockIdx.x) < ctas;
-  if (warp == 3) {   // the requests' lengths, checked once
-    int bad = 0;
-    for (int r = blockIdx.x * 32 + lane; r < P.num_seqs; r += gridDim.x * 32) load_seq(P, r, &bad);
-    if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_RECORD);
-  }
+  gr::pdl_wait();      // the plan is complete
+  const bool busy = P.run[blockIdx.x].u < P.run[blockIdx.x + 1].u;
   // registers of the two-tile kernel: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168, what the launch has
   if (warp < 4) {
     if constexpr (S::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 3) {
-      schedule_role<S>(P, sh, ctas);
+    if (warp == 3 && busy) {
+      schedule_role<S>(P, sh);
     } else if (warp == 0 && busy) {
       load_role<S, true>(P, sh, base, &mq, &mk);
     } else if (warp == 2 && busy) {
       load_role<S, false>(P, sh, base, &mq, &mv);
     } else if (warp == 1 && busy) {
-      if (lane == 0) mma_role<S, kBf16>(P, sh, base);
-      __syncwarp();
+      mma_role<S, kBf16>(P, sh, base);
       if (*reinterpret_cast<volatile int*>(&sh->abort)) {   // products in flight finish before the tensor memory goes
         if (lane == 0) tc_commit(&sh->drain);
         __syncwarp();
@@ -1022,93 +1099,6 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   if (threadIdx.x == 0 && sh->abort && P.err) atomicOr(P.err, GR_DEVERR_TIMEOUT);
   if (warp == 2) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem));
-  }
-}
-
-// ---------------------------------------------------------------- join
-// One grid column per run border: the first border inside a (block, head) joins
-// all its parts, in run order, with weights 2^(lse_i - max).  A warp takes eight
-// rows, four lanes each; the headers, the log-sums and then up to four parts'
-// columns at a time are loaded together: the kernel is a few memory latencies long.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr int kJoinRows = 8 * kJoinWarps;
-
-template <int DP, int NQ, bool kBf16>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params P, int ctas) {
-  gr::pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x + 1;
-  const Hdr h = P.hdr[c];
-  const int64_t before = P.hdr[c - 1].u0;
-  int parts = 2;                             // runs c - 1, c and those behind that start in the pair
-  for (int i = c + 1;; i += 32) {
-    const bool in = i + lane < ctas && P.hdr[min(i + lane, ctas - 1)].u0 < h.end;
-    const int n = __popc(__ballot_sync(0xFFFFFFFFu, in));
-    parts += n;
-    if (n < 32) break;
-  }
-  if (!h.mid || before > h.beg + kCost) return;
-  const int rows = h.ntok * P.group;
-  for (int r0 = blockIdx.y * kJoinRows + warp * 8; r0 < rows; r0 += gridDim.y * kJoinRows) {
-    const int r = min(r0 + (lane & 7), rows - 1), quarter = lane >> 3;
-    const bool live = r0 + (lane & 7) < rows;
-    const int tok = r / P.group, g = r - tok * P.group;
-    const int slot = tok / P.tp;
-    const int m_row = (tok - slot * P.tp) * P.group + g;
-    // the first part lies in its run's second place, the others in their first
-    const auto at = [&](int i) { return (static_cast<int64_t>(c - 1 + i) * 2 + (i == 0 ? 1 : 0)) * NQ + slot; };
-    // the row's four lanes share the log-sums
-    float top = -kInf;
-    for (int i = quarter; i < parts; i += 4) top = fmaxf(top, P.part_lse[at(i) * kRows + m_row]);
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-    const float ref = top == -kInf ? 0.0f : top;
-    float sum = 0.0f;
-    float4 acc[DP / 16];
-#pragma unroll
-    for (int x = 0; x < DP / 16; ++x) acc[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int kAhead = DP == 256 ? 1 : 2;
-    for (int i = 0; i < parts; i += kAhead) {
-      float4 v[kAhead][DP / 16];
-      float w[kAhead];
-#pragma unroll
-      for (int y = 0; y < kAhead; ++y) {
-        const int j = min(i + y, parts - 1);
-        w[y] = i + y < parts ? P.part_lse[at(j) * kRows + m_row] : -kInf;
-        const float4* o = P.part_o + (at(j) * (DP / 4) + quarter) * kRows + m_row;
-#pragma unroll
-        for (int x = 0; x < DP / 16; ++x) v[y][x] = o[x * 4 * kRows];
-      }
-#pragma unroll
-      for (int y = 0; y < kAhead; ++y) {
-        if (i + y >= parts) break;
-        const float wy = gr::fast_exp2(w[y] - ref);
-        sum += wy;
-#pragma unroll
-        for (int x = 0; x < DP / 16; ++x) {
-          acc[x].x += wy * v[y][x].x;
-          acc[x].y += wy * v[y][x].y;
-          acc[x].z += wy * v[y][x].z;
-          acc[x].w += wy * v[y][x].w;
-        }
-      }
-    }
-    if (!live) continue;
-    const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    const int64_t t = static_cast<int64_t>(h.tok0) + tok;
-    const int head = h.kvh * P.group + g;
-    unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + head * P.out_head) * 2;
-#pragma unroll
-    for (int x = 0; x < DP / 16; ++x) {
-      const int col = x * 16 + quarter * 4;
-      if (col < P.dim)
-        *reinterpret_cast<uint2*>(orow + col * 2) =
-            make_uint2(pack16<kBf16>(acc[x].x * inv, acc[x].y * inv), pack16<kBf16>(acc[x].z * inv, acc[x].w * inv));
-    }
-    if (quarter == 0 && P.lse)
-      P.lse[t * P.heads + head] =
-          sum > 0.0f || sum != sum ? (ref + __log2f(sum)) * 0.6931471805599453f : -kInf;
   }
 }
 
@@ -1134,7 +1124,7 @@ static EncodeFn encode_fn() {
 }
 
 struct Geometry {
-  int dp, nq, bn, group, tp, box, longest;
+  int dp, nq, bn, group, tp, box;
   int64_t max_items;
 };
 
@@ -1157,21 +1147,16 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
   g.bn = g.dp == 256 ? 64 : 128;
   g.box = 8;
   while (g.box * 2 <= g.bn && d->block_size % (g.box * 2) == 0) g.box *= 2;
-  g.longest = d->max_query_len > 0 ? d->max_query_len : 1;
   const int64_t per = static_cast<int64_t>(g.nq) * g.tp;
   g.max_items = static_cast<int64_t>(d->num_tokens) / per + d->num_seqs;
   if (g.max_items > 0x7FFFFFFF) return GR_ERR_UNSUPPORTED;
   return GR_OK;
 }
 
-static bool plan_in_cta(const gr_paged_attn_desc* d, const Geometry& g) {
-  return d->num_seqs <= kSmemPlan && g.max_items <= kSmemPlan;
-}
-
 static size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 struct Layout {
-  size_t hdr, part_lse, part_o, pre, item, count, total;
+  size_t run, flag, part_lse, part_o, pre, item, total;
 };
 static Layout layout(const gr_paged_attn_desc* d, const Geometry& g) {
   Layout l{};
@@ -1181,14 +1166,12 @@ static Layout layout(const gr_paged_attn_desc* d, const Geometry& g) {
     at += round256(n);
     return here;
   };
-  l.hdr = take(sizeof(Hdr) * kMaxCtas);
+  l.run = take(sizeof(Run) * (kMaxCtas + 1));
+  l.flag = take(sizeof(int32_t) * kMaxCtas * 8);
   l.part_lse = take(sizeof(float) * kMaxCtas * 2 * g.nq * kRows);
   l.part_o = take(sizeof(float) * static_cast<size_t>(kMaxCtas) * 2 * g.nq * kRows * g.dp);
-  if (!plan_in_cta(d, g)) {
-    l.pre = take(sizeof(int64_t) * (g.max_items + 1));
-    l.item = take(sizeof(int2) * g.max_items);
-    l.count = take(sizeof(int32_t));
-  }
+  l.pre = take(sizeof(int64_t) * (g.max_items + 1));
+  l.item = take(sizeof(int2) * g.max_items);
   l.total = at;
   return l;
 }
@@ -1233,18 +1216,10 @@ static int run(const Params& P, const Geometry& g, const CUtensorMap& mq, const 
     }
   }
   const int ctas = sms < kMaxCtas ? sms : kMaxCtas;
-  if (P.pre &&
-      launch(plan_kernel<S::BN>, dim3(1), kPlanThreads, 0, s, false, P, S::NQ * P.tp, static_cast<int>(g.max_items)) !=
-          cudaSuccess)
+  if (launch(plan_kernel<S::BN>, dim3(1), kPlanThreads, 0, s, false, P, S::NQ * P.tp, static_cast<int>(g.max_items),
+             ctas) != cudaSuccess)
     return GR_ERR_CUDA;
-  if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, P.pre != nullptr, P, mq, mk, mv) !=
-      cudaSuccess)
-    return GR_ERR_CUDA;
-  // a block's rows in one pass of the join
-  const int64_t rows = static_cast<int64_t>(g.longest < S::NQ * g.tp ? g.longest : S::NQ * g.tp) * g.group;
-  const int slices = static_cast<int>((rows + kJoinRows - 1) / kJoinRows);
-  if (ctas > 1 && launch(join_kernel<S::DP, S::NQ, kBf16>, dim3(ctas - 1, slices), kJoinThreads, 0, s, true, P,
-                         ctas) != cudaSuccess)
+  if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, true, P, mq, mk, mv) != cudaSuccess)
     return GR_ERR_CUDA;
   return GR_OK;
 }
@@ -1333,17 +1308,12 @@ extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_page
   P.flags = stall && stall[0] == '1' ? 1 : 0;
   P.scale = d->scale;
   P.scale_log2 = d->scale * gr::kLog2e;
-  P.hdr = reinterpret_cast<Hdr*>(ws + l.hdr);
+  P.run = reinterpret_cast<Run*>(ws + l.run);
+  P.flag = reinterpret_cast<int32_t*>(ws + l.flag);
   P.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
   P.part_o = reinterpret_cast<float4*>(ws + l.part_o);
-  P.pre = nullptr;
-  P.item = nullptr;
-  P.num_items = nullptr;
-  if (!plan_in_cta(d, g)) {
-    P.pre = reinterpret_cast<int64_t*>(ws + l.pre);
-    P.item = reinterpret_cast<int2*>(ws + l.item);
-    P.num_items = reinterpret_cast<int32_t*>(ws + l.count);
-  }
+  P.pre = reinterpret_cast<int64_t*>(ws + l.pre);
+  P.item = reinterpret_cast<int2*>(ws + l.item);
   const bool bf16 = d->dtype == GR_DTYPE_BF16;
   CUtensorMap mq, mk, mv;
   // a dimension of one entry takes any legal stride
