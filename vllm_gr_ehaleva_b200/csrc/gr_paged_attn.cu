@@ -21,7 +21,8 @@
 // CTA per SM), whatever the lengths (plan_kernel, one CTA, ahead).  A border that
 // falls into a short pair moves to the pair's nearer end; a longer pair is cut.
 // The CTA with a cut pair's end owns it: the others leave partial outputs and
-// log-sums in the workspace, which the owner joins in run order.  CTAs walk their
+// log-sums in the workspace, which the owner joins in run order.  Where whole
+// pairs already share out almost evenly, none is cut.  CTAs walk their
 // runs from the end, so that an owner comes to the join last and the parts that
 // it waits for came first in theirs, and it waits for lower-numbered CTAs only,
 // which never wait for it.  For beams, key tiles between the tail and the block's
@@ -70,6 +71,10 @@ constexpr int kSnap = GR_PA_SNAP;     // longest pair, in units, that is never c
 #define GR_PA_MINRUN 2
 #endif
 constexpr int kMinRun = GR_PA_MINRUN; // units that a CTA's run has at least, on average
+#ifndef GR_PA_JOIN
+#define GR_PA_JOIN 5
+#endif
+constexpr int kJoin = GR_PA_JOIN;     // what cutting costs a run, in units: with whole pairs the longest run may be this much longer
 constexpr int kSmemMax = 232448;      // shared memory a CTA may have
 constexpr float kRescale = 8.0f;      // log2 of the growth of the maximum that is let stand
 
@@ -334,6 +339,8 @@ template <int BN>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int per, int max_items, int ctas) {
   __shared__ int64_t part[33];
   __shared__ int64_t s_pre[kPlanItems + 1];
+  __shared__ int2 s_item[kPlanItems];
+  __shared__ int64_t s_border[kMaxCtas + 1];
   gr::pdl_trigger();
   for (int i = threadIdx.x; i < ctas * 8; i += kPlanThreads) P.flag[i] = 0;
   int64_t items = 0, total;
@@ -342,7 +349,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
     const int r = r0 + static_cast<int>(threadIdx.x);
     const int nb = r < P.num_seqs ? blocks_of(load_seq(P, r, &bad), per) : 0;
     const int64_t first = items + block_scan(nb, total, part);
-    for (int b = 0; b < nb && first + b < max_items; ++b) P.item[first + b] = make_int2(r, b);
+    for (int b = 0; b < nb && first + b < max_items; ++b) {
+      P.item[first + b] = make_int2(r, b);
+      if (first + b < kPlanItems) s_item[first + b] = make_int2(r, b);
+    }
     items += total;
   }
   if (bad && P.err) atomicOr(P.err, GR_DEVERR_BAD_RECORD);
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
     const int64_t i = i0 + threadIdx.x;
     int64_t u = 0;
     if (i < items) {
-      const int2 it = P.item[i];
+      const int2 it = i < kPlanItems ? s_item[i] : P.item[i];
       const Seq s = load_seq(P, it.x);
       u = static_cast<int64_t>(key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n + kCost) * P.kv_heads;
     }
@@ -369,28 +379,32 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
     if (items <= kPlanItems) s_pre[items] = units;
   }
   __syncthreads();
-  // border c; runs behind the last one of use are empty
+  // border c at the even share, or at the nearer end of the pair that it falls into
   const int64_t* pre = items <= kPlanItems ? s_pre : P.pre;
   const int64_t runs = items == 0 ? 0 : min(static_cast<int64_t>(ctas), max(units / kMinRun, static_cast<int64_t>(1)));
-  for (int c = threadIdx.x; c <= ctas; c += kPlanThreads) {
-    Run run{units, static_cast<int>(items) - 1, 0};
-    if (c < runs) {
-      int64_t u = units * c / runs;
-      int lo = 0, hi = static_cast<int>(items) - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pre[mid] <= u) lo = mid; else hi = mid - 1;
-      }
-      const int span = static_cast<int>((pre[lo + 1] - pre[lo]) / P.kv_heads);
-      if (span <= kSnap) {
-        const int off = static_cast<int>((u - pre[lo]) % span);
-        u += 2 * off < span ? -off : span - off;
-      }
-      run.u = u;
-      run.item = u > pre[lo] ? lo : lo - 1;   // the block of unit u - 1
+  Run even{units, static_cast<int>(items) - 1, 0}, whole = even;
+  const int c = threadIdx.x;
+  if (c < runs) {
+    const int64_t u = units * c / runs;
+    int lo = 0, hi = static_cast<int>(items) - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pre[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    P.run[c] = run;
+    const uint32_t span = static_cast<uint32_t>((pre[lo + 1] - pre[lo]) / P.kv_heads);
+    const uint32_t off = static_cast<uint32_t>(u - pre[lo]) % span;   // a block's units fit 32 bits
+    whole.u = u + (2 * off < span ? -static_cast<int64_t>(off) : static_cast<int64_t>(span - off));
+    even.u = span <= kSnap ? whole.u : u;
+    even.item = even.u > pre[lo] ? lo : lo - 1;   // the block of the unit before the border
+    whole.item = whole.u > pre[lo] ? lo : lo - 1;
   }
+  // the longest run of whole pairs
+  __syncthreads();
+  if (c <= ctas) s_border[c] = whole.u;
+  __syncthreads();
+  const bool longer = c < ctas && s_border[c + 1] - s_border[c] > units / max(runs, static_cast<int64_t>(1)) + kJoin;
+  const bool cut = __syncthreads_or(longer);
+  if (c <= ctas) P.run[c] = cut ? even : whole;
 }
 
 __device__ __forceinline__ int tile_at(const Work& k, int j) { return j < k.ta ? j : j - k.ta + k.tb; }
@@ -747,33 +761,39 @@ __device__ __forceinline__ void store32(const Params& P, unsigned char* row, int
   }
 }
 
-// The rows of one warp of a cut pair, joined by the CTA that has the pair's end:
-// out = sum_i 2^(lse_i - top) out_i / sum_i 2^(lse_i - top) over the parts in run
-// order.  Few rows (single tokens cut over many CTAs) have two or four lanes each.
-template <class S, bool kBf16>
-__device__ __forceinline__ bool join(const Params& P, Shared* sh, const Work& k, int slot, int warp) {
-  constexpr int DP = S::DP;
-  const int lane = threadIdx.x & 31;
-  const int cta = blockIdx.x, parts = cta - k.part0 + 1;
-  // every part's flag (bounded), 32 at a time
+// Where CTA p has left its part of a pair that another one owns.
+template <class S>
+__device__ __forceinline__ int64_t part_at(int p, int slot) {
+  return (static_cast<int64_t>(p) * 2 + 1) * S::NQ + slot;
+}
+
+// Waits (bounded) until the CTAs from part0 up to this one have left this warp's
+// rows of their parts.
+__device__ __forceinline__ bool wait_parts(const Params& P, Shared* sh, int part0, int slot, int warp) {
   bool ok = true;
   const uint64_t since = gr::global_timer_ns();
-  for (int p = k.part0 + lane; p < cta; p += 32) {
+  for (int p = part0 + (threadIdx.x & 31); p < static_cast<int>(blockIdx.x); p += 32) {
     while (ok && ld_acquire(P.flag + (p * 2 + slot) * 4 + warp) == 0)
       ok = *reinterpret_cast<volatile int*>(&sh->abort) == 0 && gr::global_timer_ns() - since < gr::kWaitLimitNs;
   }
-  if (!__all_sync(0xFFFFFFFFu, ok)) {
-    *reinterpret_cast<volatile int*>(&sh->abort) = 1;
-    return false;
-  }
-  // the warp's rows: token rows are the first lanes'
-  const int rows = min(min(k.nt - slot * P.tp, P.tp) * P.group - warp * 32, 32);
-  const int each = rows <= 8 ? 4 : (rows <= 16 ? 2 : 1);   // lanes per row
+  if (__all_sync(0xFFFFFFFFu, ok)) return true;
+  *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+  return false;
+}
+
+// The join of a warp of at most 16 rows (single tokens, often cut over many
+// CTAs): two or four lanes a row, this CTA's part read back from its place 0.
+template <class S, bool kBf16>
+__device__ __forceinline__ void join_few(const Params& P, const Work& k, int slot, int warp, int rows) {
+  constexpr int DP = S::DP;
+  const int lane = threadIdx.x & 31;
+  const int cta = blockIdx.x, parts = cta - k.part0 + 1;
+  const int each = rows <= 8 ? 4 : 2;   // lanes per row
   const int r = lane % (32 / each), q = lane / (32 / each);
   const int m_row = warp * 32 + min(r, rows - 1);
-  const auto place = [&](int i) {   // part i: the other CTAs' place 1, this one's place 0
+  const auto place = [&](int i) {
     const int p = k.part0 + i;
-    return (static_cast<int64_t>(p) * 2 + (p == cta ? 0 : 1)) * S::NQ + slot;
+    return p == cta ? static_cast<int64_t>(p) * 2 * S::NQ + slot : part_at<S>(p, slot);
   };
   float top = -kInf;
   for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(P.part_lse + place(i) * kRows + m_row));
@@ -782,7 +802,7 @@ __device__ __forceinline__ bool join(const Params& P, Shared* sh, const Work& k,
   const int64_t t = static_cast<int64_t>(k.q0) + k.t0 + slot * P.tp + ti;
   const int h = k.kvh * P.group + g;
   unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
-  constexpr int kAhead = 2;
+  constexpr int kAhead = 4;
   for (int x = q * 32; x < DP; x += each * 32) {
     float4 acc[8];
 #pragma unroll
@@ -793,9 +813,8 @@ __device__ __forceinline__ bool join(const Params& P, Shared* sh, const Work& k,
       float w[kAhead];
 #pragma unroll
       for (int z = 0; z < kAhead; ++z) {
-        if (i + z >= parts) break;
-        const int64_t at = place(i + z);
-        w[z] = __ldcg(P.part_lse + at * kRows + m_row);
+        const int64_t at = place(min(i + z, parts - 1));
+        w[z] = i + z < parts ? __ldcg(P.part_lse + at * kRows + m_row) : -kInf;
 #pragma unroll
         for (int y = 0; y < 8; ++y) v[z][y] = __ldcg(P.part_o + (at * (DP / 4) + x / 4 + y) * kRows + m_row);
       }
@@ -823,7 +842,6 @@ __device__ __forceinline__ bool join(const Params& P, Shared* sh, const Work& k,
         P.lse[t * P.heads + h] = sum > 0.0f || sum != sum ? (ref + __log2f(sum)) * kLn2 : -kInf;
     }
   }
-  return true;
 }
 
 // The n lowest bits (none for n <= 0, all for n >= 32).
@@ -964,18 +982,36 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
     if (!wait(sh, &sh->pv_done[lb], ((pvphase >> lb) & 1u) ^ 1u)) return;
     tc_fence_after();
     if (S::NQ == 1) step += n;
-    const bool whole = k.j0 == 0 && k.j1 == k.n;
     const bool owner = k.j0 > 0 && k.j1 == k.n;
-    // a cut pair's part goes to place 1 of this CTA, where its owner looks for it; the owner's
-    // own part to place 0
-    const int64_t place = (static_cast<int64_t>(blockIdx.x) * 2 + (owner ? 0 : 1)) * S::NQ + slot;
+    bool done = k.j0 == 0 && k.j1 == k.n;                  // this CTA stores the rows' outputs
     if (any_live) {
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      const float lse2 = l > 0.0f || l != l ? m * c + __log2f(l) : -kInf;
+      const int rows = min(min(k.nt - slot * P.tp, P.tp) * P.group - warp * 32, 32);   // the warp's first lanes
+      const int parts = owner ? static_cast<int>(blockIdx.x) - k.part0 : 0;            // other CTAs' parts
+      float scale = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      float lse2 = l > 0.0f || l != l ? m * c + __log2f(l) : -kInf;
+      float ref = 0.0f, norm = 0.0f;                       // of the join: weight of part p is 2^(lse_p - ref) norm
+      if (owner && !wait_parts(P, sh, k.part0, slot, warp)) return;
+      const bool direct = owner && rows > 16;              // rows stay with their lanes
+      if (direct) {
+        float top = lse2;
+        for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(P.part_lse + part_at<S>(k.part0 + i, slot) * kRows + m_row));
+        ref = top == -kInf ? 0.0f : top;
+        const float own = gr::fast_exp2(lse2 - ref);
+        float sum = own;
+        for (int i = 0; i < parts; ++i)
+          sum += gr::fast_exp2(__ldcg(P.part_lse + part_at<S>(k.part0 + i, slot) * kRows + m_row) - ref);
+        norm = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        scale *= own * norm;
+        lse2 = sum > 0.0f || sum != sum ? ref + __log2f(sum) : -kInf;
+        done = true;
+      }
       const int64_t t = static_cast<int64_t>(k.q0) + tok;
       const int h = k.kvh * P.group + g;
+      // a cut pair's part goes to place 1 of this CTA, where its owner looks for it; an owner's
+      // own part to place 0
+      const int64_t place = (static_cast<int64_t>(blockIdx.x) * 2 + (owner ? 0 : 1)) * S::NQ + slot;
       if (live) {
-        if (whole) {
+        if (done) {
           if (P.lse) P.lse[t * P.heads + h] = lse2 * kLn2;
         } else {
           P.part_lse[place * kRows + m_row] = lse2;
@@ -995,32 +1031,52 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->o_free[slot]);
         }
+#pragma unroll
+        for (int x = 0; x < kCols / 32; ++x)
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[x][y] = __float_as_uint(__uint_as_float(o[x][y]) * scale);
+        for (int i = 0; direct && i < parts; ++i) {
+          const int64_t at = part_at<S>(k.part0 + i, slot);
+          const float wgt = gr::fast_exp2(__ldcg(P.part_lse + at * kRows + m_row) - ref) * norm;
+          const float4* from = P.part_o + (at * (DP / 4) + x0 / 4) * kRows + m_row;
+#pragma unroll
+          for (int x = 0; x < kCols / 32; x += 2) {
+            float4 v[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y) v[y] = __ldcg(from + (x * 8 + y) * kRows);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              uint32_t* to = &o[x + y / 8][y % 8 * 4];
+              to[0] = __float_as_uint(fmaf(wgt, v[y].x, __uint_as_float(to[0])));
+              to[1] = __float_as_uint(fmaf(wgt, v[y].y, __uint_as_float(to[1])));
+              to[2] = __float_as_uint(fmaf(wgt, v[y].z, __uint_as_float(to[2])));
+              to[3] = __float_as_uint(fmaf(wgt, v[y].w, __uint_as_float(to[3])));
+            }
+          }
+        }
         if (!live) continue;
 #pragma unroll
         for (int x = 0; x < kCols / 32; ++x) {
-          if (whole) {
-            float4 v[8];
+          float4 v[8];
 #pragma unroll
-            for (int y = 0; y < 8; ++y)
-              v[y] = make_float4(__uint_as_float(o[x][4 * y]) * inv, __uint_as_float(o[x][4 * y + 1]) * inv,
-                                 __uint_as_float(o[x][4 * y + 2]) * inv, __uint_as_float(o[x][4 * y + 3]) * inv);
+          for (int y = 0; y < 8; ++y)
+            v[y] = make_float4(__uint_as_float(o[x][4 * y]), __uint_as_float(o[x][4 * y + 1]),
+                               __uint_as_float(o[x][4 * y + 2]), __uint_as_float(o[x][4 * y + 3]));
+          if (done) {
             store32<kBf16>(P, orow, x0 + x * 32, v);
           } else {
 #pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              prt[(x0 + x * 32 + y) / 4 * kRows] =
-                  make_float4(__uint_as_float(o[x][y]) * inv, __uint_as_float(o[x][y + 1]) * inv,
-                              __uint_as_float(o[x][y + 2]) * inv, __uint_as_float(o[x][y + 3]) * inv);
+            for (int y = 0; y < 8; ++y) prt[(x0 / 4 + x * 8 + y) * kRows] = v[y];
           }
         }
       }
-      if (!whole) {
+      if (!done) {
         __threadfence();
         __syncwarp();
-        if (!owner) {
-          if (lane == 0) st_release(P.flag + (blockIdx.x * 2 + slot) * 4 + warp, 1);
-        } else if (!join<S, kBf16>(P, sh, k, slot, warp)) {
-          return;
+        if (owner) {
+          join_few<S, kBf16>(P, k, slot, warp, rows);
+        } else if (lane == 0) {
+          st_release(P.flag + (blockIdx.x * 2 + slot) * 4 + warp, 1);
         }
       }
     } else {
