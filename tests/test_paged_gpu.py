@@ -371,7 +371,7 @@ def test_expired_waits_report_and_return(monkeypatch):
 
 
 # ---------------------------------------------------------------- block tables and slot maps
-@pytest.mark.parametrize("R,bs", [(1, 16), (5, 1), (37, 16), (1023, 16), (1024, 32), (1025, 48), (3000, 16)])
+@pytest.mark.parametrize("R,bs", [(1, 16), (5, 1), (37, 16), (1024, 32), (2047, 16), (2048, 32), (2049, 48), (5000, 16)])
 def test_block_tables(R, bs):
     rng = np.random.default_rng(R)
     cached = rng.integers(0, 200, R) * (rng.random(R) < 0.8)
@@ -384,7 +384,7 @@ def test_block_tables(R, bs):
     table = np.full((R, width), -1, np.int32)
     for r in range(R):
         table[r, :have[r]] = ids[:have[r]]
-    free = rng.permutation(100000).astype(np.int32)[:int((need - have).sum()) + 5]
+    free = rng.permutation(300000).astype(np.int32)[:int((need - have).sum()) + 5]
     for pad in (0, 13):
         n = int(fresh.sum()) + pad
         want = ref.extend_block_tables(table, cached, fresh, free, bs, n)

@@ -34,19 +34,18 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(fn, name, device, *args):
-    """Calls an entry point on the device's current stream, with the device current."""
-    index = device.index
+def _call(fn, name, index, *args):
+    """Calls an entry point on device `index`'s current stream, with the device current."""
     if index == torch.cuda.current_device():
         rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args, _stream(index))
     if rc != _lib.GR_OK:
         raise RuntimeError(f"{name} failed: {_lib.STATUS_NAMES.get(rc, rc)}")
 
 
-def _ints(name, t, device, dtype, shape=None):
+def _check_ints(name, t, device, dtype, shape=None):
     """An index tensor as the library reads it."""
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor on {device}")
@@ -54,10 +53,9 @@ def _ints(name, t, device, dtype, shape=None):
         raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
 
 
-def _table(block_table, device, num_seqs):
+def _check_table(block_table, device, num_seqs):
     if block_table.dtype != _I32 or block_table.device != device or block_table.dim() != 2:
         raise ValueError(f"block_table must be a 2-D int32 tensor on {device}")
     if block_table.shape[0] != num_seqs:
@@ -66,7 +64,13 @@ def _table(block_table, device, num_seqs):
         raise ValueError("block_table rows must have unit stride")
     if num_seqs > 1 and block_table.stride(0) < block_table.shape[1]:
         raise ValueError("block_table rows must not overlap")
-    return block_table.data_ptr()
+
+
+def _check_caches(k_cache, v_cache):
+    if k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("k_cache / v_cache must be [num_blocks, block_size, num_kv_heads, head_dim]")
+    if k_cache.dtype != v_cache.dtype or k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
+        raise ValueError("k_cache and v_cache must have the same dtype, shape and device")
 
 
 def _err(err, device):
@@ -77,10 +81,42 @@ def _err(err, device):
     return err.data_ptr()
 
 
-def _cuda(t, name):
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    return t.device
+class _Descs:
+    """Descriptors of calls by everything but their tensors' addresses (shapes, strides,
+    types, devices, options): a call like an earlier one skips the checks and the struct,
+    which take longer on the host than the smallest steps on the device."""
+
+    def __init__(self):
+        self.known = {}
+
+    def get(self, key, make, *args):
+        d = self.known.get(key)
+        if d is None:
+            d = make(*args)
+            if len(self.known) >= 1024:
+                self.known.clear()
+            self.known[key] = d
+        return d
+
+
+_table_descs, _store_descs, _attn_descs = _Descs(), _Descs(), _Descs()
+
+
+def _table_desc(block_table, cached_lens, new_lens, free_blocks, block_size, num_tokens):
+    if not block_table.is_cuda:
+        raise ValueError("block_table must be a CUDA tensor")
+    device, n = block_table.device, int(num_tokens)
+    if cached_lens.dim() != 1:
+        raise ValueError("cached_lens must be 1-D")
+    R = cached_lens.shape[0]
+    if int(block_size) < 1 or n < 0 or n > 0x7FFFFFFF or free_blocks.dim() != 1:
+        raise ValueError("block_size must be positive, num_tokens between 0 and 2^31 - 1, free_blocks 1-D")
+    _check_table(block_table, device, R)
+    _check_ints("cached_lens", cached_lens, device, _I32, (R,))
+    _check_ints("new_lens", new_lens, device, _I32, (R,))
+    _check_ints("free_blocks", free_blocks, device, _I32)
+    d = _lib.BlockTableDesc(R, n, free_blocks.numel(), int(block_size), block_table.shape[1], 0, block_table.stride(0))
+    return d, R, n, device.index
 
 
 def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_size: int, num_tokens: int, *, err=None):
@@ -98,35 +134,43 @@ def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_s
     (the blocks the step needs: what the caller removes from its free list).  A block that
     the free list or a row has no room for gives slot -1 and GR_DEVERR_NO_BLOCK in `err`
     (optional int32 device tensor), bad lengths GR_DEVERR_BAD_RECORD."""
-    device = _cuda(block_table, "block_table")
-    R, n = int(cached_lens.shape[0]) if cached_lens.dim() == 1 else -1, int(num_tokens)
-    if R < 0:
-        raise ValueError("cached_lens must be 1-D")
-    if int(block_size) < 1 or n < 0 or n > 0x7FFFFFFF or free_blocks.dim() != 1:
-        raise ValueError("block_size must be positive, num_tokens between 0 and 2^31 - 1, free_blocks 1-D")
-    d = _lib.BlockTableDesc(R, n, free_blocks.numel(), int(block_size), 0, 0, 0)
-    table = _table(block_table, device, R)
-    d.max_blocks, d.table_stride = block_table.shape[1], block_table.stride(0)
-    cached = _ints("cached_lens", cached_lens, device, _I32, (R,))
-    fresh = _ints("new_lens", new_lens, device, _I32, (R,))
-    free = _ints("free_blocks", free_blocks, device, _I32)
-    err = _err(err, device)
-    lib = _lib.load()
-    ints = torch.empty(2 * R + 2, dtype=_I32, device=device)
-    longs = torch.empty((2, n), dtype=_I64, device=device)
+    key = (block_table.shape, block_table.stride(), block_table.device, block_table.dtype, cached_lens.shape,
+           cached_lens.stride(), cached_lens.dtype, cached_lens.device, new_lens.shape, new_lens.stride(), new_lens.dtype,
+           new_lens.device, free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_blocks.device, block_size,
+           num_tokens)
+    d, R, n, index = _table_descs.get(key, _table_desc, block_table, cached_lens, new_lens, free_blocks, block_size,
+                                      num_tokens)
+    err = _err(err, block_table.device)
+    ints = block_table.new_empty(2 * R + 2)
+    longs = block_table.new_empty((2, n), dtype=_I64)
     at, to = ints.data_ptr(), longs.data_ptr()
-    _call(lib.gr_extend_block_tables, "gr_extend_block_tables", device, d, table, cached, fresh, free, at,
-          at + 4 * (R + 1), to, to + 8 * n, at + 4 * (2 * R + 1), err)
+    _call(_lib.load().gr_extend_block_tables, "gr_extend_block_tables", index, d, block_table.data_ptr(),
+          cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), at, at + 4 * (R + 1), to, to + 8 * n,
+          at + 4 * (2 * R + 1), err)
     cu, lens, used = ints.split_with_sizes((R + 1, R, 1))
     slots, positions = longs.unbind(0)
     return {"cu_seqlens_q": cu, "seq_lens": lens, "slot_mapping": slots, "positions": positions, "blocks_used": used}
 
 
-def _check_caches(k_cache, v_cache):
-    if k_cache.dim() != 4 or v_cache.dim() != 4:
-        raise ValueError("k_cache / v_cache must be [num_blocks, block_size, num_kv_heads, head_dim]")
-    if k_cache.dtype != v_cache.dtype or k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
-        raise ValueError("k_cache and v_cache must have the same dtype, shape and device")
+def _store_desc(k, v, k_cache, v_cache, slot_mapping):
+    if not k_cache.is_cuda:
+        raise ValueError("k_cache must be a CUDA tensor")
+    device = k_cache.device
+    _check_caches(k_cache, v_cache)
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != k_cache.shape[2:]:
+        raise ValueError("k and v must be [num_tokens, num_kv_heads, head_dim] with the cache's heads and head_dim")
+    if k.dtype != k_cache.dtype or v.dtype != k_cache.dtype or k.device != device or v.device != device:
+        raise ValueError("k and v must have the cache's dtype and device")
+    if k_cache.element_size() not in (1, 2, 4):
+        raise ValueError(f"unsupported KV element size {k_cache.element_size()}")
+    T = k.shape[0]
+    _check_ints("slot_mapping", slot_mapping, device, _I64, (T,))
+    if k.numel() and not k_cache.numel():
+        raise ValueError("the cache has no blocks")
+    nb, bs, heads, dim = k_cache.shape
+    d = _lib.KvStoreDesc(T, nb, bs, heads, dim, k_cache.element_size(), *k.stride(), *v.stride(), *k_cache.stride(),
+                         *v_cache.stride())
+    return d, device.index, k.numel() > 0
 
 
 def store_kv(k, v, k_cache, v_cache, slot_mapping, *, err=None) -> None:
@@ -136,28 +180,64 @@ def store_kv(k, v, k_cache, v_cache, slot_mapping, *, err=None) -> None:
     GR_DEVERR_BAD_SLOT in `err`.  The slots of one call must differ.  Any strides; 1-, 2- and
     4-byte elements; rows are copied as they are, so k and the cache have one dtype.  The
     inverse of extract_suffix_kv."""
-    device = _cuda(k_cache, "k_cache")
-    _check_caches(k_cache, v_cache)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != k_cache.shape[2:]:
-        raise ValueError("k and v must be [num_tokens, num_kv_heads, head_dim] with the cache's heads and head_dim")
-    if k.dtype != k_cache.dtype or v.dtype != k_cache.dtype or k.device != device or v.device != device:
-        raise ValueError("k and v must have the cache's dtype and device")
-    if k_cache.element_size() not in (1, 2, 4):
-        raise ValueError(f"unsupported KV element size {k_cache.element_size()}")
-    T = k.shape[0]
     if slot_mapping.dtype == _I32:
         slot_mapping = slot_mapping.to(_I64)
-    slots = _ints("slot_mapping", slot_mapping, device, _I64, (T,))
-    err = _err(err, device)
-    if T == 0 or k.shape[1] == 0 or k.shape[2] == 0:
-        return
-    nb, bs, heads, dim = k_cache.shape
-    if nb == 0 or bs == 0:
-        raise ValueError("the cache has no blocks")
-    d = _lib.KvStoreDesc(T, nb, bs, heads, dim, k_cache.element_size(), *k.stride(), *v.stride(), *k_cache.stride(),
-                         *v_cache.stride())
-    _call(_lib.load().gr_store_kv, "gr_store_kv", device, d, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
-          v_cache.data_ptr(), slots, err)
+    key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, k_cache.shape, k_cache.stride(),
+           k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+           slot_mapping.shape, slot_mapping.stride(), slot_mapping.dtype, slot_mapping.device)
+    d, index, any_rows = _store_descs.get(key, _store_desc, k, v, k_cache, v_cache, slot_mapping)
+    err = _err(err, k_cache.device)
+    if any_rows:
+        _call(_lib.load().gr_store_kv, "gr_store_kv", index, d, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
+              v_cache.data_ptr(), slot_mapping.data_ptr(), err)
+
+
+def _attn_desc(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seqlen_q, scale, causal, beam_tail,
+               beam_steps, out):
+    if not q.is_cuda:
+        raise ValueError("q must be a CUDA tensor")
+    device = q.device
+    _check_caches(k_cache, v_cache)
+    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype:
+        raise ValueError(f"q and the caches must both be bf16 or f16, not {q.dtype} and {k_cache.dtype}")
+    if q.dim() != 3 or q.shape[2] != k_cache.shape[3] or k_cache.device != device:
+        raise ValueError("q must be [num_tokens, num_heads, head_dim] with the cache's head_dim and device")
+    T, H, D = q.shape
+    nb, bs, HK, _ = k_cache.shape
+    if H == 0 or HK == 0 or D == 0 or bs == 0 or H % HK:
+        raise ValueError(f"num_heads={H} must be a multiple of num_kv_heads={HK}, sizes positive")
+    if D > 1 and (q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise ValueError("q and the caches need unit stride in head_dim")
+    if seq_lens.dim() != 1:
+        raise ValueError("seq_lens must be 1-D")
+    R = seq_lens.shape[0]
+    _check_ints("seq_lens", seq_lens, device, _I32)
+    _check_ints("cu_seqlens_q", cu_seqlens_q, device, _I32, (R + 1,))
+    _check_table(block_table, device, R)
+    if (beam_tail is None) != (beam_steps is None):
+        raise ValueError("beam_tail and beam_steps go together")
+    if beam_tail is not None:
+        if not causal:
+            raise ValueError("beams need causal attention")
+        _check_ints("beam_tail", beam_tail, device, _I32, (R,))
+        _check_ints("beam_steps", beam_steps, device, _I32, (R,))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, not {scale}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or
+                            (D > 1 and out.stride(2) != 1)):
+        raise ValueError("out must have q's shape, dtype and device and unit stride in head_dim")
+    out_tok, out_head = (H * D, D) if out is None else out.stride()[:2]
+    d = _lib.PagedAttnDesc(R, T, H, HK, D, bs, block_table.shape[1], _DTYPES[q.dtype], int(bool(causal)),
+                           int(max_seqlen_q), scale, 0, nb, block_table.stride(0), q.stride(0), q.stride(1),
+                           *k_cache.stride()[:3], *v_cache.stride()[:3], out_tok, out_head)
+    size = ctypes.c_size_t(0)
+    _lib.check(_lib.load().gr_paged_attention_workspace_size(d, size), "gr_paged_attention_workspace_size")
+    return d, size.value, device.index, bool(T and R)
+
+
+def _kind(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seqlen_q: int, *, scale=None,
@@ -188,51 +268,24 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, ma
     16-byte aligned tensors.  Block ids outside the cache read as zero rows and set
     GR_DEVERR_BAD_SLOT in `err` (optional int32 device tensor); lengths outside the table's
     row or the tokens are clamped and set GR_DEVERR_BAD_RECORD."""
-    device = _cuda(q, "q")
-    _check_caches(k_cache, v_cache)
-    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype:
-        raise ValueError(f"q and the caches must both be bf16 or f16, not {q.dtype} and {k_cache.dtype}")
-    if q.dim() != 3 or q.shape[2] != k_cache.shape[3] or k_cache.device != device:
-        raise ValueError("q must be [num_tokens, num_heads, head_dim] with the cache's head_dim and device")
-    T, H, D = q.shape
-    nb, bs, HK, _ = k_cache.shape
-    if H == 0 or HK == 0 or D == 0 or bs == 0 or H % HK:
-        raise ValueError(f"num_heads={H} must be a multiple of num_kv_heads={HK}, sizes positive")
-    if D > 1 and (q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
-        raise ValueError("q and the caches need unit stride in head_dim")
-    if seq_lens.dim() != 1:
-        raise ValueError("seq_lens must be 1-D")
-    R = seq_lens.shape[0]
-    io = _lib.PagedAttnIO()
-    io.seq_lens = _ints("seq_lens", seq_lens, device, _I32)
-    io.cu_seqlens = _ints("cu_seqlens_q", cu_seqlens_q, device, _I32, (R + 1,))
-    io.block_table = _table(block_table, device, R)
-    if (beam_tail is None) != (beam_steps is None):
-        raise ValueError("beam_tail and beam_steps go together")
-    if beam_tail is not None:
-        if not causal:
-            raise ValueError("beams need causal attention")
-        io.beam_tail = _ints("beam_tail", beam_tail, device, _I32, (R,))
-        io.beam_steps = _ints("beam_steps", beam_steps, device, _I32, (R,))
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, not {scale}")
+    key = (q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+           v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, block_table.shape, block_table.stride(),
+           block_table.dtype, block_table.device, cu_seqlens_q.shape, cu_seqlens_q.stride(), cu_seqlens_q.dtype,
+           cu_seqlens_q.device, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, max_seqlen_q, scale,
+           causal, _kind(beam_tail), _kind(beam_steps), _kind(out))
+    d, size, index, any_rows = _attn_descs.get(key, _attn_desc, q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens,
+                                               max_seqlen_q, scale, causal, beam_tail, beam_steps, out)
+    err = _err(err, q.device)
     if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or (D > 1 and out.stride(2) != 1):
-        raise ValueError("out must have q's shape, dtype and device and unit stride in head_dim")
-    lse = torch.empty((T, H), dtype=torch.float32, device=device) if return_lse else None
-    d = _lib.PagedAttnDesc(R, T, H, HK, D, bs, block_table.shape[1], _DTYPES[q.dtype], int(bool(causal)),
-                           int(max_seqlen_q), scale, 0, nb, block_table.stride(0), q.stride(0), q.stride(1),
-                           *k_cache.stride()[:3], *v_cache.stride()[:3], out.stride(0), out.stride(1))
-    lib = _lib.load()
-    size = ctypes.c_size_t(0)
-    _lib.check(lib.gr_paged_attention_workspace_size(d, size), "gr_paged_attention_workspace_size")
-    io.err = _err(err, device)
-    if T and R:
+        out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    if any_rows:
         # from the caching allocator per call: stream ordered, and a captured graph keeps its own
-        ws = torch.empty(size.value, dtype=torch.uint8, device=device)
-        io.q, io.k_cache, io.v_cache, io.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-        io.lse = None if lse is None else lse.data_ptr()
-        _call(lib.gr_paged_attention, "gr_paged_attention", device, d, io, ws.data_ptr(), size.value)
+        ws = q.new_empty(size, dtype=torch.uint8)
+        io = _lib.PagedAttnIO(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                              cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
+                              None if beam_tail is None else beam_tail.data_ptr(),
+                              None if beam_steps is None else beam_steps.data_ptr(), out.data_ptr(),
+                              None if lse is None else lse.data_ptr(), err)
+        _call(_lib.load().gr_paged_attention, "gr_paged_attention", index, d, io, ws.data_ptr(), size)
     return (out, lse) if return_lse else out

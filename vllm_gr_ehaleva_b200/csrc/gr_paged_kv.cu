@@ -3,7 +3,7 @@
 //
 // extend_block_tables_kernel.  Two exclusive sums over the requests (new
 // tokens, blocks taken) decide everything else, and they are short: every CTA
-// computes them for itself, 1024 requests at a time in shared memory, and then
+// computes them for itself, 2048 requests at a time in shared memory, and then
 // writes its even share of the tile's requests, fresh blocks and tokens, each
 // found by a binary search in the sums.  So the step is one launch without a
 // grid-wide wait, and a batch of one long chunk spreads over the grid as well
@@ -28,7 +28,7 @@ namespace grpk {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTile = 1024;                    // requests per pass of the table kernel
+constexpr int kTile = 2048;                    // requests per pass of the table kernel
 constexpr int kPerThread = kTile / kThreads;
 
 struct TableParams {
