@@ -59,22 +59,10 @@ using gr::smem_u32;
 constexpr int kRows = 128;            // rows of a query tile (the matrix product's M)
 constexpr int kMaxCtas = 160;
 constexpr int kWorkRing = 4;          // (block, head) pairs handed out ahead
-#ifndef GR_PA_COST
-#define GR_PA_COST 2
-#endif
-constexpr int kCost = GR_PA_COST;     // what a pair costs besides its key tiles, in key tiles
-#ifndef GR_PA_SNAP
-#define GR_PA_SNAP 8
-#endif
-constexpr int kSnap = GR_PA_SNAP;     // longest pair, in units, that is never cut
-#ifndef GR_PA_MINRUN
-#define GR_PA_MINRUN 2
-#endif
-constexpr int kMinRun = GR_PA_MINRUN; // units that a CTA's run has at least, on average
-#ifndef GR_PA_JOIN
-#define GR_PA_JOIN 5
-#endif
-constexpr int kJoin = GR_PA_JOIN;     // what cutting costs a run, in units: with whole pairs the longest run may be this much longer
+constexpr int kCost = 2;     // what a pair costs besides its key tiles, in key tiles
+constexpr int kSnap = 8;     // longest pair, in units, that is never cut
+constexpr int kMinRun = 2; // units that a CTA's run has at least, on average
+constexpr int kJoin = 5;     // what cutting costs a run, in units: with whole pairs the longest run may be this much longer
 constexpr int kSmemMax = 232448;      // shared memory a CTA may have
 constexpr float kRescale = 8.0f;      // log2 of the growth of the maximum that is let stand
 
@@ -244,10 +232,16 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
 }
 
 // A wait by a whole warp.  One that gives up sets the CTA's abort flag, which
-// ends every other wait; the warp's lanes leave together or not at all.
+// ends every other wait; the warp's lanes leave together or not at all.  The
+// limit is a number of tries: reading the timer between them, or trying more
+// often, takes issue slots from the warps that are waited for (beams 614 k
+// cycles with the timer, 575 k without, 770 k with a spin of test_wait).
+constexpr int kTries = 500000;    // about 2 s: a try that fails sleeps some 4 us
 __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity) {
-  const bool ok = gr::mbar_wait_bounded(bar, parity, &sh->abort);
-  if (__all_sync(0xFFFFFFFFu, ok)) return true;
+  for (int i = 0; i < kTries; ++i) {
+    if (__all_sync(0xFFFFFFFFu, gr::mbar_try_wait(bar, parity))) return true;
+    if (*reinterpret_cast<volatile int*>(&sh->abort)) break;
+  }
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
 }
