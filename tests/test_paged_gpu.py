@@ -206,6 +206,14 @@ def test_results_do_not_depend_on_the_run():
     assert got is out and torch.equal(out, o1)
 
 
+def test_the_query_bound_only_picks_the_kernel():
+    # a bound below the longest query and one far above: the other kernel, the same rows
+    for D in (64, 128):
+        b = Batch([500, 30, 0], [1, 150, 70], 8, 2, D, 16, BF16, seed=26)
+        for bound in (0, 1, 10 ** 9):
+            b.check(*b.run(max_new=bound))
+
+
 def test_scale():
     b = Batch([200], [130], 4, 2, 128, 16, BF16, seed=19)
     b.check(*b.run(scale=0.3), scale=0.3)
@@ -312,6 +320,57 @@ def test_sizes_of_zero():
     for kc, tab in ((k[:0], np.zeros((1, 1))), (k, np.zeros((1, 0)))):
         out, lse = paged_attention(q, kc, kc, _i32(tab), _i32([0, 3]), _i32([0]), 3, return_lse=True)
         assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_refusals():
+    b = Batch([20, 3], [2, 1], 4, 2, 64, 16, BF16, seed=27)
+    t, cu, lens = _i32(b.table), _i32(b.cu), _i32(b.lens)
+
+    def call(q=b.q, k=b.k, v=b.v, t=t, cu=cu, lens=lens, n=2, **kw):
+        return paged_attention(q, k, v, t, cu, lens, n, **kw)
+
+    want = call()
+    wide = torch.zeros(3, 4, 72, dtype=BF16, device=DEV)
+    for match, kw in (
+            ("bf16 or f16", dict(q=b.q.float())), ("bf16 or f16", dict(q=b.q.half())),
+            ("same dtype", dict(v=b.v.half())), ("num_blocks, block_size", dict(k=b.k[0], v=b.v[0])),
+            ("head_dim", dict(q=wide)), ("multiple of", dict(q=b.q[:, :3])), ("unit stride", dict(q=b.q.transpose(0, 2).contiguous().transpose(0, 2))),
+            ("int32", dict(lens=lens.long())), ("int32", dict(cu=cu.long())), ("int32", dict(t=t.long())),
+            ("shape", dict(cu=cu[:2])), ("rows for", dict(t=t[:1])), ("1-D", dict(lens=lens[None])),
+            ("unit stride", dict(t=torch.zeros(2, 6, dtype=torch.int32, device=DEV)[:, ::2])),
+            ("contiguous", dict(lens=torch.zeros(4, dtype=torch.int32, device=DEV)[::2])),
+            ("int32", dict(lens=lens.cpu())), ("CUDA", dict(q=b.q.cpu())),
+            ("go together", dict(beam_tail=lens)), ("go together", dict(beam_steps=lens)),
+            ("causal", dict(beam_tail=lens, beam_steps=lens, causal=False)),
+            ("scale", dict(scale=0.0)), ("scale", dict(scale=-1)), ("scale", dict(scale=float("nan"))),
+            ("scale", dict(scale=float("inf"))), ("out must", dict(out=torch.empty_like(b.q).half())),
+            ("out must", dict(out=torch.empty_like(b.q)[:2])), ("err must", dict(err=lens.long()))):
+        with pytest.raises(ValueError, match=match):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="GR_ERR_MISALIGNED"):
+        call(q=torch.zeros(3 * 4 * 64 + 1, dtype=BF16, device=DEV)[1:].view(3, 4, 64))
+    with pytest.raises(RuntimeError, match="GR_ERR_MISALIGNED"):
+        call(out=torch.zeros(3, 4, 68, dtype=BF16, device=DEV)[..., :64])
+    with pytest.raises(RuntimeError, match="GR_ERR_UNSUPPORTED"):
+        call(k=b.k.view(-1, 4, 2, 64), v=b.v.view(-1, 4, 2, 64))
+    with pytest.raises(RuntimeError, match="GR_ERR_BAD_DESC"):
+        call(n=-1)
+    assert torch.equal(call(), want)
+
+    s = torch.arange(3, device=DEV)
+    k = torch.zeros(3, 2, 64, dtype=BF16, device=DEV)
+    for match, args in (("cache's heads", (k[:, :1], k[:, :1], b.k, b.v, s)), ("dtype", (k.half(), k.half(), b.k, b.v, s)),
+                        ("shape", (k, k, b.k, b.v, s[:2])), ("int64", (k, k, b.k, b.v, s.float())),
+                        ("no blocks", (k, k, b.k[:0], b.v[:0], s)), ("element size", (k.double(), k.double(), b.k.double(), b.v.double(), s)),
+                        ("CUDA", (k, k, b.k.cpu(), b.v.cpu(), s))):
+        with pytest.raises(ValueError, match=match):
+            store_kv(*args)
+    for match, args in (("rows for", (t, lens[:1], lens[:1], lens, 16, 3)), ("shape", (t, lens, lens[:1], lens, 16, 3)),
+                        ("int32", (t, lens, lens, lens.long(), 16, 3)), ("positive", (t, lens, lens, lens, 0, 3)),
+                        ("num_tokens", (t, lens, lens, lens, 16, -1)), ("1-D", (t, lens[None], lens, lens, 16, 3)),
+                        ("overlap", (torch.zeros(4, dtype=torch.int32, device=DEV).as_strided((2, 3), (1, 1)), lens, lens, lens, 16, 3))):
+        with pytest.raises(ValueError, match=match):
+            extend_block_tables(*args)
 
 
 def test_captured_beside_eager_calls_and_on_another_stream():

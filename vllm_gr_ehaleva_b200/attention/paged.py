@@ -105,17 +105,17 @@ _table_descs, _store_descs, _attn_descs = _Descs(), _Descs(), _Descs()
 def _table_desc(block_table, cached_lens, new_lens, free_blocks, block_size, num_tokens):
     if not block_table.is_cuda:
         raise ValueError("block_table must be a CUDA tensor")
-    device, n = block_table.device, int(num_tokens)
+    device, n = block_table.device, num_tokens
     if cached_lens.dim() != 1:
         raise ValueError("cached_lens must be 1-D")
     R = cached_lens.shape[0]
-    if int(block_size) < 1 or n < 0 or n > 0x7FFFFFFF or free_blocks.dim() != 1:
+    if block_size < 1 or n < 0 or n > 0x7FFFFFFF or free_blocks.dim() != 1:
         raise ValueError("block_size must be positive, num_tokens between 0 and 2^31 - 1, free_blocks 1-D")
     _check_table(block_table, device, R)
     _check_ints("cached_lens", cached_lens, device, _I32, (R,))
     _check_ints("new_lens", new_lens, device, _I32, (R,))
     _check_ints("free_blocks", free_blocks, device, _I32)
-    d = _lib.BlockTableDesc(R, n, free_blocks.numel(), int(block_size), block_table.shape[1], 0, block_table.stride(0))
+    d = _lib.BlockTableDesc(R, n, free_blocks.numel(), block_size, block_table.shape[1], 0, block_table.stride(0))
     return d, R, n, device.index
 
 
@@ -134,6 +134,7 @@ def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_s
     (the blocks the step needs: what the caller removes from its free list).  A block that
     the free list or a row has no room for gives slot -1 and GR_DEVERR_NO_BLOCK in `err`
     (optional int32 device tensor), bad lengths GR_DEVERR_BAD_RECORD."""
+    block_size, num_tokens = int(block_size), int(num_tokens)
     key = (block_table.shape, block_table.stride(), block_table.device, block_table.dtype, cached_lens.shape,
            cached_lens.stride(), cached_lens.dtype, cached_lens.device, new_lens.shape, new_lens.stride(), new_lens.dtype,
            new_lens.device, free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_blocks.device, block_size,
@@ -221,15 +222,15 @@ def _attn_desc(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seq
             raise ValueError("beams need causal attention")
         _check_ints("beam_tail", beam_tail, device, _I32, (R,))
         _check_ints("beam_steps", beam_steps, device, _I32, (R,))
-    scale = D ** -0.5 if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else scale
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, not {scale}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or
                             (D > 1 and out.stride(2) != 1)):
         raise ValueError("out must have q's shape, dtype and device and unit stride in head_dim")
     out_tok, out_head = (H * D, D) if out is None else out.stride()[:2]
-    d = _lib.PagedAttnDesc(R, T, H, HK, D, bs, block_table.shape[1], _DTYPES[q.dtype], int(bool(causal)),
-                           int(max_seqlen_q), scale, 0, nb, block_table.stride(0), q.stride(0), q.stride(1),
+    d = _lib.PagedAttnDesc(R, T, H, HK, D, bs, block_table.shape[1], _DTYPES[q.dtype], int(causal),
+                           max_seqlen_q, scale, 0, nb, block_table.stride(0), q.stride(0), q.stride(1),
                            *k_cache.stride()[:3], *v_cache.stride()[:3], out_tok, out_head)
     size = ctypes.c_size_t(0)
     _lib.check(_lib.load().gr_paged_attention_workspace_size(d, size), "gr_paged_attention_workspace_size")
@@ -268,6 +269,9 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, ma
     16-byte aligned tensors.  Block ids outside the cache read as zero rows and set
     GR_DEVERR_BAD_SLOT in `err` (optional int32 device tensor); lengths outside the table's
     row or the tokens are clamped and set GR_DEVERR_BAD_RECORD."""
+    # a longer bound than any query tile picks the same kernel
+    max_seqlen_q, causal = min(int(max_seqlen_q), 129), bool(causal)
+    scale = None if scale is None else float(scale)
     key = (q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
            v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, block_table.shape, block_table.stride(),
            block_table.dtype, block_table.device, cu_seqlens_q.shape, cu_seqlens_q.stride(), cu_seqlens_q.dtype,
