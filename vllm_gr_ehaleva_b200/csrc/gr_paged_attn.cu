@@ -77,7 +77,10 @@ struct Shape {
   static constexpr int kQTile = CH * kChunkQ;
   static constexpr int kStage = CH * kChunkKV;
   static constexpr int kStages = DP == 64 ? 10 : (NQ == 2 || DP == 256 ? 5 : 6);
-  static constexpr int kThreads = 128 + 128 * NQ;
+  // warps 0..3: loads, products, loads, schedule; kNQ = 1: four more that load; then the softmax
+  static constexpr int kLoaders = NQ == 2 ? 1 : 3;     // warps that load keys (as many load values)
+  static constexpr int kSoftmax = NQ == 2 ? 4 : 8;     // first softmax warp
+  static constexpr int kThreads = 32 * kSoftmax + 128 * NQ;
   static constexpr int kColO = 2 * BN;                 // tensor memory: S0, S1, O0, (O1)
   static constexpr int kData = NQ * kQTile + kStages * kStage;
   static_assert(kColO + NQ * DP <= 512, "tensor memory columns");
@@ -109,8 +112,8 @@ struct Shared {
 };
 
 struct Run {                       // where a CTA's run starts
-  int64_t u;                       // in units of the batch
-  int32_t item, pad;               // the query block that the run before it ends in
+  int64_t u;                       // in units of the batch, KV heads outermost
+  int32_t head, item;              // the pair that the run before it ends in
 };
 
 struct Params {
@@ -132,8 +135,9 @@ struct Params {
   int flags;                       // 1: copies are not issued (test hook)
   float scale_log2, scale;
   // plan and partials in the workspace
-  int64_t* pre;                    // [items + 1] units before each query block
+  int64_t* pre;                    // [items + 1] units of one KV head before each query block
   int2* item;                      // request, block
+  int32_t* items;                  // how many
   Run* run;                        // [ctas + 1]
   int32_t* flag;                   // [ctas][2][4] part written (query tile, warp of it)
   float4* part_o;                  // [ctas][2][NQ][DP / 4][128 rows]: a warp's stores of its 32 rows are whole lines
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
     if (i < items) {
       const int2 it = i < kPlanItems ? s_item[i] : P.item[i];
       const Seq s = load_seq(P, it.x);
-      u = static_cast<int64_t>(key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n + kCost) * P.kv_heads;
+      u = key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n + kCost;
     }
     const int64_t ex = block_scan(u, total, part);
     if (i < items) {
@@ -370,33 +374,42 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
   }
   if (threadIdx.x == 0) {
     P.pre[items] = units;
+    P.items[0] = static_cast<int>(items);
     if (items <= kPlanItems) s_pre[items] = units;
   }
   __syncthreads();
   // border c at the even share, or at the nearer end of the pair that it falls into
   const int64_t* pre = items <= kPlanItems ? s_pre : P.pre;
-  const int64_t runs = items == 0 ? 0 : min(static_cast<int64_t>(ctas), max(units / kMinRun, static_cast<int64_t>(1)));
-  Run even{units, static_cast<int>(items) - 1, 0}, whole = even;
+  const int64_t all = units * P.kv_heads;
+  const int64_t runs = items == 0 ? 0 : min(static_cast<int64_t>(ctas), max(all / kMinRun, static_cast<int64_t>(1)));
+  Run even{all, P.kv_heads - 1, static_cast<int>(items) - 1}, whole = even;
   const int c = threadIdx.x;
   if (c < runs) {
-    const int64_t u = units * c / runs;
+    const int64_t u = all * c / runs;
+    const int head = static_cast<int>(u / units);
+    const int64_t in = u - head * units;
     int lo = 0, hi = static_cast<int>(items) - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] <= u) lo = mid; else hi = mid - 1;
+      if (pre[mid] <= in) lo = mid; else hi = mid - 1;
     }
-    const uint32_t span = static_cast<uint32_t>((pre[lo + 1] - pre[lo]) / P.kv_heads);
-    const uint32_t off = static_cast<uint32_t>(u - pre[lo]) % span;   // a block's units fit 32 bits
-    whole.u = u + (2 * off < span ? -static_cast<int64_t>(off) : static_cast<int64_t>(span - off));
+    const int64_t span = pre[lo + 1] - pre[lo], off = in - pre[lo];
+    whole.u = u - off + (2 * off < span ? 0 : span);
     even.u = span <= kSnap ? whole.u : u;
-    even.item = even.u > pre[lo] ? lo : lo - 1;   // the block of the unit before the border
-    whole.item = whole.u > pre[lo] ? lo : lo - 1;
+    // the pair of the unit before the border
+    const auto before = [&](Run& r) {
+      const bool here = r.u > u - off;
+      r.head = here || lo > 0 ? head : head - 1;
+      r.item = here ? lo : (lo > 0 ? lo - 1 : static_cast<int>(items) - 1);
+    };
+    before(even);
+    before(whole);
   }
   // the longest run of whole pairs
   __syncthreads();
   if (c <= ctas) s_border[c] = whole.u;
   __syncthreads();
-  const bool longer = c < ctas && s_border[c + 1] - s_border[c] > units / max(runs, static_cast<int64_t>(1)) + kJoin;
+  const bool longer = c < ctas && s_border[c + 1] - s_border[c] > all / max(runs, static_cast<int64_t>(1)) + kJoin;
   const bool cut = __syncthreads_or(longer);
   if (c <= ctas) P.run[c] = cut ? even : whole;
 }
@@ -438,7 +451,12 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
   int64_t u = stop.u;
   const int per = S::NQ * P.tp;
   uint32_t seq = 0;
-  for (int i = stop.item; u > begin; --i) {
+  int64_t beg = u;                                   // of the pair; its last unit is the run's last one
+  for (int i = stop.item, head = stop.head; u > begin; --i) {
+    if (i < 0) {
+      --head;
+      i = P.items[0] - 1;
+    }
     const int2 it = P.item[i];
     const Seq s = load_seq(P, it.x);
     Work k;
@@ -451,37 +469,29 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
     k.t0 = it.y * per;
     k.nt = min(s.n - k.t0, per);
     k.slots = k.nt > P.tp ? 2 : 1;
+    k.kvh = head;
     const Tiles t = key_tiles<S::BN>(s, P.causal, k.t0, k.t0 + k.nt);
     k.ta = t.a;
     k.tb = t.b;
     k.n = t.n;
     const int span = t.n + kCost;
-    const int64_t base = P.pre[i];
-    k.kvh = P.kv_heads - 1;
-    int hi = span;                                   // end of the run in the pair
-    const int64_t in = u - base;
-    if (in < static_cast<int64_t>(span) * P.kv_heads) {
-      k.kvh = static_cast<int>((in - 1) / span);
-      hi = static_cast<int>(in - static_cast<int64_t>(k.kvh) * span);
+    beg = seq == 0 && u == stop.u ? head * P.pre[P.items[0]] + P.pre[i] : u - span;
+    const int hi = static_cast<int>(u - beg);        // end of the run in the pair
+    const int lo = static_cast<int>(max(begin - beg, static_cast<int64_t>(0)));
+    k.j0 = max(lo - kCost, 0);
+    k.j1 = max(hi - kCost, 0);
+    u = beg + lo;
+    if (k.j1 <= k.j0) continue;
+    k.part0 = blockIdx.x;
+    if (k.j0 > 0 && k.j1 == k.n)                     // this CTA joins the parts
+      do --k.part0; while (k.part0 > 0 && P.run[k.part0].u > beg + kCost);
+    const int at = seq % kWorkRing;
+    if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
+    if (lane == 0) {
+      sh->work[at] = k;
+      mbar_arrive(&sh->wk_full[at]);
     }
-    for (; k.kvh >= 0 && u > begin; --k.kvh, hi = span) {
-      const int64_t beg = u - hi;
-      const int lo = static_cast<int>(max(begin - beg, static_cast<int64_t>(0)));
-      k.j0 = max(lo - kCost, 0);
-      k.j1 = max(hi - kCost, 0);
-      u = beg + lo;
-      if (k.j1 <= k.j0) continue;
-      k.part0 = blockIdx.x;
-      if (k.j0 > 0 && k.j1 == k.n)                   // this CTA joins the parts
-        do --k.part0; while (k.part0 > 0 && P.run[k.part0].u > beg + kCost);
-      const int at = seq % kWorkRing;
-      if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
-      if (lane == 0) {
-        sh->work[at] = k;
-        mbar_arrive(&sh->wk_full[at]);
-      }
-      ++seq;
-    }
+    ++seq;
   }
   const int at = seq % kWorkRing;
   if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
@@ -491,14 +501,15 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
   }
 }
 
-// Warp 0: the block's queries once, then its key tiles; warp 2: its value tiles.
+// Warp 0: the block's queries once, then its key tiles; warp 2: its value tiles;
+// `part` of the warps that share the tiles' copies (an issue takes some 100 cycles,
+// and single tokens over blocks of 16 rows need 32 copies per 2 x 32 KB).
 // Tiles take the ring's stages in the order in which the products first use them:
 // K0 .. K(lead-1), V0, K(lead), V1, ...  A lane looks up one copy's block a tile
-// ahead, one lane issues the copies (lanes issuing their own took 100 cycles a
-// copy, and blocks of 16 rows make 32 copies of a key and a value tile).
+// ahead, one lane issues the copies.
 template <class S, bool kKeys>
 __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t data, const CUtensorMap* mq,
-                                          const CUtensorMap* map) {
+                                          const CUtensorMap* map, int part) {
   const int lane = threadIdx.x & 31;
   Work k;
   Ring<S> ring;
@@ -510,7 +521,7 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
   constexpr int kLead = S::NQ == 2 ? 1 : 2;
   int bad = 0;
   while (ok && next_work(sh, seq, k)) {
-    if (kKeys) {
+    if (kKeys && part == 0) {
       if (!wait(sh, &sh->q_empty, qphase ^ 1u)) break;
       if (lane == 0 && !(P.flags & 1)) {
         const int slots = S::NQ == 2 ? k.slots : 1;
@@ -549,10 +560,10 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
         break;
       }
       if (!(P.flags & 1)) {
-        if (lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
+        if (part == 0 && lane == 0) mbar_arrive_expect_tx(&sh->full[ring.stage], S::kStage);
         mine |= 1u << ring.stage;
         const uint32_t dst = ringbase + ring.stage * S::kStage;
-        for (int i = 0; i < boxes; ++i) {
+        for (int i = part; i < boxes; i += S::kLoaders) {
           const int b = __shfl_sync(0xFFFFFFFFu, id0, i), r = __shfl_sync(0xFFFFFFFFu, off0, i);
           if (lane == 0) {
 #pragma unroll
@@ -1096,7 +1107,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     }
     for (int i = 0; i < kWorkRing; ++i) {
       mbar_init(&sh->wk_full[i], 1);
-      mbar_init(&sh->wk_empty[i], 3 + 4 * S::NQ);
+      mbar_init(&sh->wk_empty[i], 2 * S::kLoaders + 1 + 4 * S::NQ);
     }
     mbar_init(&sh->q_full, 1);
     mbar_init(&sh->q_empty, 1);
@@ -1121,26 +1132,38 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 
   gr::pdl_wait();      // the plan is complete
   const bool busy = P.run[blockIdx.x].u < P.run[blockIdx.x + 1].u;
-  // registers of the two-tile kernel: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168, what the launch has
-  if (warp < 4) {
-    if constexpr (S::NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 3 && busy) {
+  // registers: 12 warps of 168 at launch give 4 x 56 + 8 x 224 (kNQ = 2), and 8 x 80 + 4 x 240 leave some (kNQ = 1)
+  static_assert(S::kThreads == 384, "register split");
+  if (warp < S::kSoftmax) {
+    if constexpr (S::NQ == 2) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    }
+    if (!busy) {
+    } else if (warp == 3) {
       schedule_role<S>(P, sh);
-    } else if (warp == 0 && busy) {
-      load_role<S, true>(P, sh, base, &mq, &mk);
-    } else if (warp == 2 && busy) {
-      load_role<S, false>(P, sh, base, &mq, &mv);
-    } else if (warp == 1 && busy) {
+    } else if (warp == 1) {
       mma_role<S, kBf16>(P, sh, base);
       if (*reinterpret_cast<volatile int*>(&sh->abort)) {   // products in flight finish before the tensor memory goes
         if (lane == 0) tc_commit(&sh->drain);
         __syncwarp();
         gr::mbar_wait_bounded(&sh->drain, 0);
       }
+    } else if (warp & 1) {
+      load_role<S, false>(P, sh, base, &mq, &mv, warp / 2 - 1);   // 5, 7
+    } else if (warp == 2) {
+      load_role<S, false>(P, sh, base, &mq, &mv, 0);
+    } else {
+      load_role<S, true>(P, sh, base, &mq, &mk, warp / 2 - (warp > 0));   // 0, 4, 6
     }
   } else {
-    if constexpr (S::NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    if (busy) softmax_role<S, kBf16>(P, sh, base, (warp >> 2) - 1);
+    if constexpr (S::NQ == 2) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
+    }
+    if (busy) softmax_role<S, kBf16>(P, sh, base, (warp - S::kSoftmax) >> 2);
   }
   __syncwarp();
   tc_fence_before();
@@ -1206,7 +1229,7 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
 static size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 struct Layout {
-  size_t run, flag, part_lse, part_o, pre, item, total;
+  size_t run, flag, part_lse, part_o, pre, item, items, total;
 };
 static Layout layout(const gr_paged_attn_desc* d, const Geometry& g) {
   Layout l{};
@@ -1222,6 +1245,7 @@ static Layout layout(const gr_paged_attn_desc* d, const Geometry& g) {
   l.part_o = take(sizeof(float) * static_cast<size_t>(kMaxCtas) * 2 * g.nq * kRows * g.dp);
   l.pre = take(sizeof(int64_t) * (g.max_items + 1));
   l.item = take(sizeof(int2) * g.max_items);
+  l.items = take(sizeof(int32_t));
   l.total = at;
   return l;
 }
@@ -1364,6 +1388,7 @@ extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_page
   P.part_o = reinterpret_cast<float4*>(ws + l.part_o);
   P.pre = reinterpret_cast<int64_t*>(ws + l.pre);
   P.item = reinterpret_cast<int2*>(ws + l.item);
+  P.items = reinterpret_cast<int32_t*>(ws + l.items);
   const bool bf16 = d->dtype == GR_DTYPE_BF16;
   CUtensorMap mq, mk, mv;
   // a dimension of one entry takes any legal stride
