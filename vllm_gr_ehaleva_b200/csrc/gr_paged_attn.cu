@@ -70,12 +70,14 @@ template <int DP_, int NQ_>
 struct Shape {
   static constexpr int DP = DP_;                       // head dim, padded to 64 / 128 / 256
   static constexpr int NQ = NQ_;                       // query tiles per block
-  static constexpr int BN = DP == 256 ? 64 : 128;      // keys per tile
+  static constexpr int BN = 128;                       // keys per tile
   static constexpr int CH = DP / 64;                   // 128-byte column chunks of a row
+  static constexpr int SUB = DP == 256 ? 2 : 1;        // ring stages per tile: 128 columns each
+  static constexpr int CHS = CH / SUB;                 // chunks of a stage
   static constexpr int kChunkQ = kRows * 128;          // bytes of one chunk of a query tile
   static constexpr int kChunkKV = BN * 128;
   static constexpr int kQTile = CH * kChunkQ;
-  static constexpr int kStage = CH * kChunkKV;
+  static constexpr int kStage = CHS * kChunkKV;
   static constexpr int kStages = DP == 64 ? 10 : (NQ == 2 || DP == 256 ? 5 : 6);
   // warps 0..3: loads, products, loads, schedule; kNQ = 1: four more that load; then the softmax
   static constexpr int kLoaders = NQ == 2 ? 1 : 3;     // warps that load keys (as many load values)
@@ -549,12 +551,14 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
     };
     int id, off;
     look(0, id, off);
-    for (int x = 0, ki = 0, vi = 0; x < 2 * n; ++x, ring.next()) {
-      const bool is_k = ki < n && ki < vi + kLead;
-      const int j = is_k ? ki++ : vi++;
+    for (int x = 0, ki = 0, vi = 0; x < 2 * S::SUB * n; ++x, ring.next()) {
+      // (key and value stages, SUB to a tile)
+      const bool is_k = ki < n * S::SUB && ki / S::SUB < vi / S::SUB + kLead && (vi % S::SUB == 0 || ki % S::SUB != 0);
+      const int js = is_k ? ki++ : vi++;
       if (is_k != kKeys) continue;
+      const int j = js / S::SUB, sub = js % S::SUB;
       const int id0 = id, off0 = off;
-      if (j + 1 < n) look(j + 1, id, off);
+      if (sub == S::SUB - 1 && j + 1 < n) look(j + 1, id, off);
       if (!wait(sh, &sh->empty[ring.stage], ring.phase ^ 1u)) {
         ok = false;
         break;
@@ -567,8 +571,9 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
           const int b = __shfl_sync(0xFFFFFFFFu, id0, i), r = __shfl_sync(0xFFFFFFFFu, off0, i);
           if (lane == 0) {
 #pragma unroll
-            for (int c = 0; c < S::CH; ++c)
-              tma_load4(dst + c * S::kChunkKV + i * P.box * 128, map, c * 64, k.kvh, r, b, &sh->full[ring.stage]);
+            for (int c = 0; c < S::CHS; ++c)
+              tma_load4(dst + c * S::kChunkKV + i * P.box * 128, map, (sub * S::CHS + c) * 64, k.kvh, r, b,
+                        &sh->full[ring.stage]);
           }
         }
       }
@@ -607,30 +612,30 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
   // fp32 accumulators, A and B of one type, M = 128; B of the second product is stored along N
   constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((S::BN / 8) << 17) | ((kRows / 16) << 24);
   constexpr uint32_t kIdescO =
-      (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((S::DP / 8) << 17) | ((kRows / 16) << 24);
+      (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((S::CHS * 64 / 8) << 17) | ((kRows / 16) << 24);
 
-  const auto qk = [&](int q, int buf, int stage) {   // S[buf] = Q[q] K^T
-    const uint64_t qa = smem_desc(data + q * S::kQTile, 16, 1024);
+  const auto qk = [&](int q, int buf, int stage, int sub) {   // S[buf] (+)= Q[q] K^T over the stage's columns
+    const uint64_t qa = smem_desc(data + q * S::kQTile + sub * S::CHS * S::kChunkQ, 16, 1024);
     const uint64_t ka = smem_desc(ringbase + stage * S::kStage, 16, 1024);
     if (leader) {
 #pragma unroll
-      for (int c = 0; c < S::CH; ++c)
+      for (int c = 0; c < S::CHS; ++c)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
           tc_mma_ss(tmem + buf * S::BN, qa + ((c * S::kChunkQ + x * 32) >> 4), ka + ((c * S::kChunkKV + x * 32) >> 4),
-                    kIdescS, (c | x) != 0);
+                    kIdescS, (sub | c | x) != 0);
     }
-    commit(&sh->s_full[buf]);
+    if (sub == S::SUB - 1) commit(&sh->s_full[buf]);
   };
-  const auto pv = [&](int q, int buf, int stage, bool first) {   // O[q] (+)= P[buf] V
+  const auto pv = [&](int q, int buf, int stage, bool first, int sub) {   // the stage's columns of O[q] (+)= P[buf] V
     const uint64_t va = smem_desc(ringbase + stage * S::kStage, S::kChunkKV, 1024);
     if (leader) {
 #pragma unroll
       for (int x = 0; x < S::BN / 16; ++x)
-        tc_mma_ts(tmem + S::kColO + q * S::DP, tmem + buf * S::BN + x * 8, va + ((x * 2048) >> 4), kIdescO,
-                  !(first && x == 0));
+        tc_mma_ts(tmem + S::kColO + q * S::DP + sub * S::CHS * 64, tmem + buf * S::BN + x * 8, va + ((x * 2048) >> 4),
+                  kIdescO, !(first && x == 0));
     }
-    commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
+    if (sub == S::SUB - 1) commit(&sh->pv_done[S::NQ == 2 ? q : buf]);
   };
 
   Ring<S> ring;
@@ -665,7 +670,7 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
     int kstage = 0, vstage = 0;
     if (S::NQ == 2) {
       if (!take(kstage)) return;
-      for (int q = 0; q < slots; ++q) qk(q, q, kstage);
+      for (int q = 0; q < slots; ++q) qk(q, q, kstage, 0);
       commit(&sh->empty[kstage]);
       if (n == 1) commit(&sh->q_empty);
       for (int j = 0; j < n; ++j) {
@@ -675,11 +680,11 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
           if (j == 0 && !o_free(q)) return;
           if (!probs(q)) return;
           tc_fence_after();
-          pv(q, q, vstage, j == 0);
+          pv(q, q, vstage, j == 0, 0);
           if (last) commit(&sh->empty[vstage]);
           if (j + 1 < n) {
             if (q == 0 && !take(kstage)) return;
-            qk(q, q, kstage);
+            qk(q, q, kstage, 0);
             if (last) {
               commit(&sh->empty[kstage]);
               if (j + 2 == n) commit(&sh->q_empty);
@@ -688,10 +693,17 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
         }
       }
     } else {
+      const auto keys = [&](int buf) {
+#pragma unroll
+        for (int sub = 0; sub < S::SUB; ++sub) {
+          if (!take(kstage)) return false;
+          qk(0, buf, kstage, sub);
+          commit(&sh->empty[kstage]);
+        }
+        return true;
+      };
       for (int j = 0; j < 2 && j < n; ++j) {
-        if (!take(kstage)) return;
-        qk(0, (step + j) & 1, kstage);
-        commit(&sh->empty[kstage]);
+        if (!keys((step + j) & 1)) return;
         if (j + 1 == n) commit(&sh->q_empty);
       }
       for (int j = 0; j < n; ++j, ++step) {
@@ -700,12 +712,16 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
         if (j == 0 && !o_free(0)) return;
         if (!probs(b)) return;
         tc_fence_after();
-        pv(0, b, vstage, j == 0);
+        pv(0, b, vstage, j == 0, 0);
         commit(&sh->empty[vstage]);
+#pragma unroll
+        for (int sub = 1; sub < S::SUB; ++sub) {
+          if (!take(vstage)) return;
+          pv(0, b, vstage, j == 0, sub);
+          commit(&sh->empty[vstage]);
+        }
         if (j + 2 < n) {
-          if (!take(kstage)) return;
-          qk(0, b, kstage);
-          commit(&sh->empty[kstage]);
+          if (!keys(b)) return;
           if (j + 3 == n) commit(&sh->q_empty);
         }
       }
@@ -719,7 +735,7 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
 template <class S>
 __device__ __forceinline__ void zero_tail(uint32_t tile, int from, int to) {
   const int n = (to - from) * 8;
-  for (int e = threadIdx.x & 127; e < n * S::CH; e += 128) {
+  for (int e = threadIdx.x & 127; e < n * S::CHS; e += 128) {
     const int c = e / n, x = e - c * n;
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * S::kChunkKV + from * 128 + x * 16), "r"(0)
                  : "memory");
@@ -746,7 +762,7 @@ __device__ __forceinline__ int32_t ld_acquire(const int32_t* p) {
 
 // 32 output columns from col on, as far as the head dim goes.
 template <bool kBf16>
-__device__ __forceinline__ void store32(const Params& P, unsigned char* row, int col, const float4 (&v)[8]) {
+__device__ __forceinline__ void store32(const Params& P, unsigned char* row, int col, const float4* v) {
 #pragma unroll
   for (int y = 0; y < 2; ++y) {
     uint32_t w[8];
@@ -869,7 +885,7 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
   Work k;
   uint32_t seq = 0, sphase = 0, pvphase = 0;   // one bit per buffer
   uint32_t step = 0, tiles = 0;                // score buffer of the next step, tiles through the ring
-  for (; next_work(sh, seq, k); tiles += 2 * (k.j1 - k.j0)) {
+  for (; next_work(sh, seq, k); tiles += 2 * S::SUB * (k.j1 - k.j0)) {
     if (S::NQ == 2 && slot >= k.slots) continue;
     const int n = k.j1 - k.j0;
     // this row: token, position, the keys it sees
@@ -969,12 +985,15 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
         l += x0 + x1;
       }
       if (j == n - 1 && slot == 0) {
-        // the pair's last value tile is the last in the ring so far
+        // the pair's last value tile takes the last stages in the ring so far
         const int rows = k.len - key0;
         if (rows > 0 && rows < BN && rows % P.box != 0) {
-          const uint32_t pos = tiles + 2 * n - 1, stage = pos % S::kStages;
-          if (!wait(sh, &sh->full[stage], (pos / S::kStages) & 1u)) return;
-          zero_tail<S>(data + S::NQ * S::kQTile + stage * S::kStage, rows, (rows / P.box + 1) * P.box);
+#pragma unroll
+          for (int sub = 0; sub < S::SUB; ++sub) {
+            const uint32_t pos = tiles + 2 * S::SUB * n - S::SUB + sub, stage = pos % S::kStages;
+            if (!wait(sh, &sh->full[stage], (pos / S::kStages) & 1u)) return;
+            zero_tail<S>(data + S::NQ * S::kQTile + stage * S::kStage, rows, (rows / P.box + 1) * P.box);
+          }
         }
       }
       tc_fence_before();
@@ -1024,57 +1043,59 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
       }
       unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
       float4* prt = P.part_o + place * (DP / 4) * kRows + m_row;
-      constexpr int kCols = DP < 128 ? DP : 128;   // columns in registers at a time
+      constexpr int kCols = 64;   // columns in registers at a time, beside those of two other parts
 #pragma unroll 1
       for (int x0 = 0; x0 < DP; x0 += kCols) {
-        uint32_t o[kCols / 32][32];
-#pragma unroll
-        for (int x = 0; x < kCols / 32; ++x) tc_ld32(o[x], o_col + x0 + x * 32);
+        uint32_t o[2][32];
+        tc_ld32(o[0], o_col + x0);
+        tc_ld32(o[1], o_col + x0 + 32);
         tc_wait_ld();
-        if (x0 + kCols >= DP) {   // read out: the next pair's products may begin
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->o_free[slot]);
+        float4 v[16];
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+          const uint32_t* from = &o[y / 8][y % 8 * 4];
+          v[y] = make_float4(__uint_as_float(from[0]) * scale, __uint_as_float(from[1]) * scale,
+                             __uint_as_float(from[2]) * scale, __uint_as_float(from[3]) * scale);
         }
+        if (direct) {
+#pragma unroll 1
+          for (int i = 0; i < parts; i += 2) {
+            float4 a[2][16];
+            float wgt[2];
 #pragma unroll
-        for (int x = 0; x < kCols / 32; ++x)
+            for (int z = 0; z < 2; ++z) {
+              const int64_t at = part_at<S>(k.part0 + min(i + z, parts - 1), slot);
+              wgt[z] = i + z < parts ? __ldcg(P.part_lse + at * kRows + m_row) : -kInf;
+              const float4* from = P.part_o + (at * (DP / 4) + x0 / 4) * kRows + m_row;
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[x][y] = __float_as_uint(__uint_as_float(o[x][y]) * scale);
-        for (int i = 0; direct && i < parts; ++i) {
-          const int64_t at = part_at<S>(k.part0 + i, slot);
-          const float wgt = gr::fast_exp2(__ldcg(P.part_lse + at * kRows + m_row) - ref) * norm;
-          const float4* from = P.part_o + (at * (DP / 4) + x0 / 4) * kRows + m_row;
+              for (int y = 0; y < 16; ++y) a[z][y] = __ldcg(from + y * kRows);
+            }
 #pragma unroll
-          for (int x = 0; x < kCols / 32; x += 2) {
-            float4 v[16];
+            for (int z = 0; z < 2; ++z) {
+              if (i + z >= parts) break;
+              const float w = gr::fast_exp2(wgt[z] - ref) * norm;
 #pragma unroll
-            for (int y = 0; y < 16; ++y) v[y] = __ldcg(from + (x * 8 + y) * kRows);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              uint32_t* to = &o[x + y / 8][y % 8 * 4];
-              to[0] = __float_as_uint(fmaf(wgt, v[y].x, __uint_as_float(to[0])));
-              to[1] = __float_as_uint(fmaf(wgt, v[y].y, __uint_as_float(to[1])));
-              to[2] = __float_as_uint(fmaf(wgt, v[y].z, __uint_as_float(to[2])));
-              to[3] = __float_as_uint(fmaf(wgt, v[y].w, __uint_as_float(to[3])));
+              for (int y = 0; y < 16; ++y) {
+                v[y].x = fmaf(w, a[z][y].x, v[y].x);
+                v[y].y = fmaf(w, a[z][y].y, v[y].y);
+                v[y].z = fmaf(w, a[z][y].z, v[y].z);
+                v[y].w = fmaf(w, a[z][y].w, v[y].w);
+              }
             }
           }
         }
         if (!live) continue;
+        if (done) {
+          store32<kBf16>(P, orow, x0, v);
+          store32<kBf16>(P, orow, x0 + 32, v + 8);
+        } else {
 #pragma unroll
-        for (int x = 0; x < kCols / 32; ++x) {
-          float4 v[8];
-#pragma unroll
-          for (int y = 0; y < 8; ++y)
-            v[y] = make_float4(__uint_as_float(o[x][4 * y]), __uint_as_float(o[x][4 * y + 1]),
-                               __uint_as_float(o[x][4 * y + 2]), __uint_as_float(o[x][4 * y + 3]));
-          if (done) {
-            store32<kBf16>(P, orow, x0 + x * 32, v);
-          } else {
-#pragma unroll
-            for (int y = 0; y < 8; ++y) prt[(x0 / 4 + x * 8 + y) * kRows] = v[y];
-          }
+          for (int y = 0; y < 16; ++y) prt[(x0 / 4 + y) * kRows] = v[y];
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->o_free[slot]);
       if (!done) {
         __threadfence();
         __syncwarp();
@@ -1217,7 +1238,7 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
   g.tp = kRows / g.group;
   // one query tile where the longest query fits it, or the accumulators of two do not
   g.nq = (g.dp == 256 || static_cast<int64_t>(d->max_query_len) <= g.tp) ? 1 : 2;
-  g.bn = g.dp == 256 ? 64 : 128;
+  g.bn = 128;
   g.box = 8;
   while (g.box * 2 <= g.bn && d->block_size % (g.box * 2) == 0) g.box *= 2;
   const int64_t per = static_cast<int64_t>(g.nq) * g.tp;
