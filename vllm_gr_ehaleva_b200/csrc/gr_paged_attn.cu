@@ -911,78 +911,102 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
       // scores, kNQ = 1 does not (the other buffer's is still to come)
       if (any_live) {
         const uint32_t s_col = tmem + b * BN;
-        uint32_t sr[BN / 32][32];
+        uint32_t sr[BN / 32][32], p[BN / 2];
+        const auto score = [&](int x) { return __uint_as_float(sr[x / 32][x % 32]); };
+        const auto load = [&] {   // the tile's scores, -inf where the row does not see the key
 #pragma unroll
-        for (int x = 0; x < BN / 32; ++x) tc_ld32(sr[x], s_col + x * 32);
-        tc_wait_ld();
-        const bool whole = key0 + BN <= lim && (key0 + BN <= first || key0 >= own);
-        if (!__all_sync(0xFFFFFFFFu, whole)) {
-          // one bit per key, then one select per score (comparisons per score
-          // made this path 5 us per tile)
+          for (int x = 0; x < BN / 32; ++x) tc_ld32(sr[x], s_col + x * 32);
+          tc_wait_ld();
+          const bool whole = key0 + BN <= lim && (key0 + BN <= first || key0 >= own);
+          if (!__all_sync(0xFFFFFFFFu, whole)) {
+            // one bit per key, then one select per score (comparisons per score
+            // made this path 5 us per tile)
 #pragma unroll
-          for (int x = 0; x < BN / 32; ++x) {
-            const uint32_t see = low_bits(lim - key0 - x * 32) &
-                                 (low_bits(first - key0 - x * 32) | ~low_bits(own - key0 - x * 32));
+            for (int x = 0; x < BN / 32; ++x) {
+              const uint32_t see = low_bits(lim - key0 - x * 32) &
+                                   (low_bits(first - key0 - x * 32) | ~low_bits(own - key0 - x * 32));
 #pragma unroll
-            for (int y = 0; y < 32; ++y) sr[x][y] = see & (1u << y) ? sr[x][y] : 0xFF800000u;
-          }
-        }
-        float t[4] = {-kInf, -kInf, -kInf, -kInf};
-#pragma unroll
-        for (int x = 0; x < BN; x += 8)
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            t[y] = max3(t[y], __uint_as_float(sr[x / 32][x % 32 + 2 * y]), __uint_as_float(sr[x / 32][x % 32 + 2 * y + 1]));
-        const float top = max3(fmaxf(t[0], t[1]), t[2], t[3]);
-        // a reference of its own for the row's first keys, then only when the growth is large
-        const bool grow = live && ((top - m) * c > kRescale || (m == -kInf && top > -kInf));
-        if (__any_sync(0xFFFFFFFFu, grow)) {
-          const float f = grow ? gr::fast_exp2((m - top) * c) : 1.0f;   // m = -inf: 0
-          if (grow) m = top;
-          if (j > 0) {
-            if (S::NQ == 1) {
-              const int pb = b ^ 1;   // the previous key tile's product
-              if (!wait(sh, &sh->pv_done[pb], ((pvphase >> pb) & 1u) ^ 1u)) return;
-              tc_fence_after();
+              for (int y = 0; y < 32; ++y) sr[x][y] = see & (1u << y) ? sr[x][y] : 0xFF800000u;
             }
-            l *= f;
-#pragma unroll 1
-            for (int x = 0; x < DP; x += 32) {
-              uint32_t o[32];
-              tc_ld32(o, o_col + x);
-              tc_wait_ld();
-#pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-              tc_st32(o_col + x, o);
-            }
-            tc_wait_st();
           }
-        }
-        const float mc = m == -kInf ? 0.0f : m * c;
-        const uint64_t c2 = gr::pack2(c, c), n2 = gr::pack2(-mc, -mc);
-        uint64_t a0 = 0, a1 = 0;   // (0.0f, 0.0f)
+        };
+        const auto maximum = [&] {
+          float t[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
-        for (int h = 0; h < BN / 64; ++h) {
-          uint32_t p[32];
+          for (int x = 0; x < BN; x += 2) t[x / 2 % 4] = max3(t[x / 2 % 4], score(x), score(x + 1));
+          return max3(fmaxf(t[0], t[1]), t[2], t[3]);
+        };
+        // p = 2^(c s - c m), rounded; returns the unrounded sum
+        const auto exponentials = [&] {
+          const float mc = m == -kInf ? 0.0f : m * c;
+          const uint64_t c2 = gr::pack2(c, c), n2 = gr::pack2(-mc, -mc);
+          uint64_t a0 = 0, a1 = 0;   // (0.0f, 0.0f)
 #pragma unroll
-          for (int x = 0; x < 64; x += 2) {
-            const int y = h * 64 + x;
-            const uint64_t t = gr::ffma2(
-                gr::pack2(__uint_as_float(sr[y / 32][y % 32]), __uint_as_float(sr[y / 32][y % 32 + 1])), c2, n2);
+          for (int x = 0; x < BN; x += 2) {
             float e0, e1;
-            gr::unpack2(t, e0, e1);
+            gr::unpack2(gr::ffma2(gr::pack2(score(x), score(x + 1)), c2, n2), e0, e1);
             e0 = gr::fast_exp2(e0);
             e1 = gr::fast_exp2(e1);
             if (x & 2) a1 = gr::fadd2(a1, gr::pack2(e0, e1)); else a0 = gr::fadd2(a0, gr::pack2(e0, e1));
             p[x / 2] = pack16<kBf16>(e0, e1);
           }
-          tc_st32(s_col + h * 32, p);
+          float x0, x1;
+          gr::unpack2(gr::fadd2(a0, a1), x0, x1);
+          return x0 + x1;
+        };
+        // a later tile's maximum becomes the reference: what is there of l and O is scaled
+        const auto rescale = [&](bool grow, float top) {
+          const float f = grow ? gr::fast_exp2((m - top) * c) : 1.0f;   // m = -inf: 0
+          if (grow) m = top;
+          l *= f;
+          if (j == 0) return true;
+          if (S::NQ == 1) {
+            const int pb = b ^ 1;   // the previous key tile's product
+            if (!wait(sh, &sh->pv_done[pb], ((pvphase >> pb) & 1u) ^ 1u)) return false;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int x = 0; x < DP; x += 32) {
+            uint32_t o[32];
+            tc_ld32(o, o_col + x);
+            tc_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            tc_st32(o_col + x, o);
+          }
+          tc_wait_st();
+          return true;
+        };
+        load();
+        float sum;
+        if constexpr (S::NQ == 2) {
+          // the maximum first: a reference for the row's first keys, then only large growth counts
+          const float top = maximum();
+          const bool grow = live && ((top - m) * c > kRescale || (m == -kInf && top > -kInf));
+          if (__any_sync(0xFFFFFFFFu, grow) && !rescale(grow, top)) return;
+          sum = exponentials();
+        } else {
+          // One group of softmax warps is the chain's slowest link: later tiles are exponentiated
+          // against the reference at hand and their maximum is taken meanwhile; where it has
+          // grown too far, which is rare, the tile is done again.  (64 single tokens 304 -> 286 k
+          // cycles; two query tiles, which fill each other's gaps, lose 1 to 3 % by it.)
+          if (__any_sync(0xFFFFFFFFu, live && m == -kInf)) {
+            const float top = maximum();
+            if (m == -kInf) m = top;   // until now l = 0 and O = 0
+          }
+          while (true) {
+            sum = exponentials();
+            const float top = maximum();
+            const bool grow = live && (top - m) * c > kRescale;
+            if (!__any_sync(0xFFFFFFFFu, grow)) break;
+            if (!rescale(grow, top)) return;
+            load();
+          }
         }
+        l += sum;
+#pragma unroll
+        for (int h = 0; h < BN / 64; ++h) tc_st32(s_col + h * 32, *reinterpret_cast<uint32_t(*)[32]>(p + h * 32));
         tc_wait_st();
-        a0 = gr::fadd2(a0, a1);
-        float x0, x1;
-        gr::unpack2(a0, x0, x1);
-        l += x0 + x1;
       }
       if (j == n - 1 && slot == 0) {
         // the pair's last value tile takes the last stages in the ring so far
