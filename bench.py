@@ -65,8 +65,9 @@ def parse():
                     help="vocab-sharded cfg5: how the lm_head's columns are dealt to the ranks")
     ap.add_argument("--catalog-cache", default=None,
                     help="directory to keep built synthetic catalogs in (reused by later runs of the same call)")
-    ap.add_argument("--component", default="step", choices=["step", "suffix_kv", "wire", "remux", "hook"],
-                    help="suffix_kv: the suffix KV gather of the attention pass; wire: the step message (host); "
+    ap.add_argument("--component", default="step", choices=["step", "suffix_kv", "paged", "wire", "remux", "hook"],
+                    help="suffix_kv: the suffix KV gather of the attention pass; paged: the paged KV cache (block "
+                         "tables, cache write, attention); wire: the step message (host); "
                          "remux: the worker's logprobs remux; hook: the worker-side step over cfg2 sessions")
     return ap.parse_args()
 
@@ -872,6 +873,82 @@ def run_suffix_kv(args):
         print(json.dumps(line), flush=True)
 
 
+# ------------------------------------------------------------------ paged KV cache
+def run_paged(args):
+    """The three calls of a step over the paged KV cache, one after the other on
+    the same batch: block tables and slot maps, cache write, attention.  Batches:
+    single tokens over long caches, one prompt, and the beams of mega requests
+    (32 query heads over 8 KV heads of 128, bf16, blocks of 16)."""
+    import torch
+    from vllm_gr_ehaleva_b200.attention import extend_block_tables, paged_attention, store_kv
+    device = torch.device("cuda", 0)
+    torch.cuda.set_device(device)
+    H, HK, D, block = 32, 8, 128, 16
+    peak, peak_kind = peaks()
+    path = os.path.join(ROOT, "MEASURED_PEAKS.json")
+    tflops = 1590.0
+    if os.path.exists(path):
+        with open(path) as f:
+            tflops = float(json.load(f)["bf16_tflops"])
+    rng = np.random.default_rng(11)
+    g = torch.Generator(device=device).manual_seed(11)
+    stream = torch.cuda.current_stream(device)
+
+    def timed(fn, iters):
+        for _ in range(max(args.warmup, 3)):
+            fn()
+        torch.cuda.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record(stream)
+        for _ in range(iters):
+            fn()
+        e1.record(stream)
+        torch.cuda.synchronize()
+        return e0.elapsed_time(e1) / iters
+
+    batches = [("single_tokens", rng.integers(500, 16384, 64), np.ones(64, np.int64), 0, 0),
+               ("prompt", np.zeros(1, np.int64), np.full(1, 8192), 0, 0),
+               ("beams", rng.integers(600, 2600, 32), np.full(32, 24 + 128 * 3), 24, 3)]
+    for name, cached, fresh, tail, steps in batches:
+        i32 = lambda x: torch.from_numpy(np.asarray(x)).to(device, torch.int32)  # noqa: E731
+        R, T, keys = len(cached), int(fresh.sum()), int((cached + fresh).sum())
+        have, need = -(-cached // block), -(-(cached + fresh) // block)
+        nb = int(need.sum()) + 8
+        ids = torch.randperm(nb, device=device, generator=g).to(torch.int32)
+        table = torch.zeros(R, int(need.max()), dtype=torch.int32, device=device)
+        table[torch.arange(table.shape[1], device=device)[None] < i32(have)[:, None]] = ids[:int(have.sum())]
+        free = ids[int(have.sum()):].clone()
+        k_cache = torch.randn(nb, block, HK, D, device=device, generator=g).to(torch.bfloat16)
+        v_cache = torch.randn(nb, block, HK, D, device=device, generator=g).to(torch.bfloat16)
+        k = torch.randn(T, HK, D, device=device, generator=g).to(torch.bfloat16)
+        q = torch.randn(T, H, D, device=device, generator=g).to(torch.bfloat16)
+        c, f = i32(cached), i32(fresh)
+        beams = dict(beam_tail=i32(np.full(R, tail)), beam_steps=i32(np.full(R, steps))) if steps else {}
+        m = extend_block_tables(table, c, f, free, block, T)
+        mx = int(fresh.max())
+        iters = min(args.steps, 100)
+        ms_t = timed(lambda: extend_block_tables(table, c, f, free, block, T), iters)
+        ms_s = timed(lambda: store_kv(k, k, k_cache, v_cache, m["slot_mapping"]), iters)
+        ms_a = timed(lambda: paged_attention(q, k_cache, v_cache, table, m["cu_seqlens_q"], m["seq_lens"], mx, **beams),
+                     iters)
+        pairs = int((fresh * cached + fresh * (fresh + 1) // 2).sum())
+        if steps:
+            w = (mx - tail) // steps
+            pairs = int((fresh * cached).sum()) + R * (tail * (tail + 1) // 2 + w * (steps * tail + steps * (steps + 1) // 2))
+        flops = 4 * H * D * pairs
+        nbytes = 4 * keys * HK * D + 4 * T * H * D
+        bound = "hbm" if nbytes / (peak * 1e9) > flops / (tflops * 1e12) else "tensor"
+        floor_ms = max(nbytes / (peak * 1e9), flops / (tflops * 1e12)) * 1e3
+        print(json.dumps({
+            "metric": "attention over the paged KV cache, time per call", "batch": name, "value": round(ms_a, 5),
+            "unit": "ms", "higher_is_better": False, "tflops": round(flops / ms_a / 1e9, 1),
+            "gbs": round(nbytes / ms_a / 1e6, 1), "block_tables_ms": round(ms_t, 5), "store_ms": round(ms_s, 5),
+            "dtype": "bf16", "config": {"requests": R, "tokens": T, "keys": keys, "heads": H, "kv_heads": HK,
+                                        "head_dim": D, "block_size": block, "beam_tail": tail, "beam_steps": steps},
+            "roofline": {"bound": bound, "floor_ms": round(floor_ms, 5), "frac": round(floor_ms / ms_a, 4),
+                         "peak_gbs": peak, "peak_tflops": tflops, "peak_kind": peak_kind}}), flush=True)
+
+
 # ------------------------------------------------------------------ step message (host)
 def run_wire(args):
     """Build + encode + decode + the core's token list for one mega-request step
@@ -1032,6 +1109,9 @@ def main():
         return
     if args.component == "suffix_kv":
         run_suffix_kv(args)
+        return
+    if args.component == "paged":
+        run_paged(args)
         return
     if args.component == "wire":
         run_wire(args)

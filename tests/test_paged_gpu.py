@@ -430,7 +430,7 @@ def test_expired_waits_report_and_return(monkeypatch):
 
 
 # ---------------------------------------------------------------- block tables and slot maps
-@pytest.mark.parametrize("R,bs", [(1, 16), (5, 1), (37, 16), (1024, 32), (2047, 16), (2048, 32), (2049, 48), (5000, 16)])
+@pytest.mark.parametrize("R,bs", [(1, 16), (5, 1), (37, 16), (256, 16), (257, 16), (1024, 32), (2047, 16), (2048, 32), (2049, 48), (5000, 16)])
 def test_block_tables(R, bs):
     rng = np.random.default_rng(R)
     cached = rng.integers(0, 200, R) * (rng.random(R) < 0.8)
