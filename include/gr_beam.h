@@ -456,7 +456,8 @@ int32_t gr_store_kv(const gr_kv_store_desc* desc, const void* k, const void* v, 
  * the paged attention kernel (beam_attn.py:734-755).
  *
  * Limits (GR_ERR_UNSUPPORTED): head_dim a multiple of 8 up to 256; block_size a
- * multiple of 8; num_heads / num_kv_heads at most 128.  Strides are in elements;
+ * multiple of 8; num_heads / num_kv_heads at most 128.  num_tokens and max_blocks *
+ * block_size at most 2^31 - 1024, num_blocks below 2^31 - 1 (GR_ERR_BAD_DESC).  Strides are in elements;
  * rows are contiguous in the head dimension, and every other stride and address
  * of q, the caches and out must be a multiple of 16 bytes (GR_ERR_MISALIGNED).
  * Block ids outside [0, num_blocks) read as zero rows and set

@@ -56,6 +56,7 @@ def _attn(**kw):
     (dict(head_dim=0), BAD), (dict(block_size=0), BAD), (dict(causal=2), BAD), (dict(max_query_len=-1), BAD),
     (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=float("nan")), BAD), (dict(scale=float("inf")), BAD),
     (dict(table_stride=3), BAD), (dict(num_blocks=2 ** 31), BAD), (dict(max_blocks=2 ** 27, table_stride=2 ** 27), BAD),
+    (dict(num_tokens=2 ** 31 - 1000), BAD), (dict(scale=3e38), BAD),
     (dict(dtype=0), DTYPE), (dict(dtype=9), DTYPE),
     (dict(head_dim=264), UNSUPPORTED), (dict(head_dim=100), UNSUPPORTED), (dict(block_size=12), UNSUPPORTED),
     (dict(num_heads=258), UNSUPPORTED),

@@ -242,6 +242,24 @@ def test_strided_queries_caches_and_outputs():
     assert (out[:, 1::2] == 7).all()
 
 
+def test_smallest_sizes():
+    # one token, one head, one block; strides of dimensions of one entry mean nothing
+    for ctx, D in ((0, 8), (5, 8), (3, 256)):
+        b = Batch([ctx], [1], 1, 1, D, 8, BF16, seed=ctx, spare=0)
+        b.check(*b.run())
+        q = b.q.as_strided((1, 1, D), (3, 5, 1))
+        k, v = (x.as_strided((1, 8, 1, D), (7, D, 3, 1)) for x in (b.k, b.v))
+        assert torch.equal(paged_attention(q, k, v, _i32(b.table), _i32(b.cu), _i32(b.lens), 1), b.run()[0])
+
+
+def test_one_request_among_many_without_tokens():
+    # plan passes of 1024 requests, most of them empty
+    new = np.zeros(3000, np.int64)
+    new[[0, 1023, 1024, 2999]] = [3, 200, 1, 70]
+    b = Batch(np.full(3000, 2), new, 4, 2, 64, 8, BF16, seed=28)
+    b.check(*b.run())
+
+
 def test_rows_of_no_request_stay():
     b = Batch([10, 20], [5, 6], 4, 2, 64, 16, BF16, seed=21)
     o, _ = b.run()

@@ -31,11 +31,18 @@
 // Kernel.  Warps 0 and 2 load keys and values (tensor-map copies of the blocks'
 // rows, 128-byte swizzle, one ring of tiles), warp 1 issues the matrix products
 // (S = Q K^T from shared memory, O += P V with P in tensor memory), warp 3 walks
-// the run and hands out its (block, head) pairs; warps 4.. are the softmax: one thread per
+// the run and hands out its pairs; the last warps are the softmax: one thread per
 // row.  Two query tiles (kNQ = 2) have a softmax group each and alternate on the
-// tensor pipe; one tile (kNQ = 1: blocks of at most 128 rows, or heads above
-// 128) alternates two score buffers instead.
-// Every wait is bounded (GR_DEVERR_TIMEOUT).
+// tensor pipe; one tile (kNQ = 1: no query of more than 128 rows, or heads above
+// 128, whose accumulators leave no room) alternates two score buffers instead and
+// has four more loading warps.  Heads above 128 move their tiles as two halves of
+// 128 columns.  Every wait is bounded (GR_DEVERR_TIMEOUT).
+//
+// Bound and measured (32 query heads over 8 KV heads of 128, blocks of 16): 64
+// single tokens over 2.5 GB of cache 6.3 TB/s, HBM, 96 % of a plain copy's rate; a
+// prompt of 8192 1080 to 1170 TFLOP/s, the chain scores - softmax - product of a
+// query tile (exponential unit and tensor pipe each near half of their rate), and
+// in long runs the power limit.
 
 #include <cstdint>
 #include <cstdlib>
@@ -59,10 +66,13 @@ using gr::smem_u32;
 constexpr int kRows = 128;            // rows of a query tile (the matrix product's M)
 constexpr int kMaxCtas = 160;
 constexpr int kWorkRing = 4;          // (block, head) pairs handed out ahead
-constexpr int kCost = 2;     // what a pair costs besides its key tiles, in key tiles
-constexpr int kSnap = 8;     // longest pair, in units, that is never cut
-constexpr int kMinRun = 2; // units that a CTA's run has at least, on average
-constexpr int kJoin = 5;     // what cutting costs a run, in units: with whole pairs the longest run may be this much longer
+// The shares of the work, in units of a key tile (about 2 us with two query tiles).  Measured on
+// 64 single tokens, a prompt of 8192, ragged chunks and beams: kCost 1 and 3, kMinRun 3 and 4,
+// kJoin 3 and 8 are within 2 % of these on each, kMinRun 4 loses 10 % on two single tokens.
+constexpr int kCost = 2;              // what a pair costs besides its key tiles
+constexpr int kSnap = 8;              // longest pair that is never cut
+constexpr int kMinRun = 2;            // what a CTA's run has at least, on average
+constexpr int kJoin = 5;              // with whole pairs the longest run may be this much longer than with cut ones
 constexpr int kSmemMax = 232448;      // shared memory a CTA may have
 constexpr float kRescale = 8.0f;      // log2 of the growth of the maximum that is let stand
 
@@ -152,6 +162,13 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of the warp, the same one every time.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(yes));
+  return yes != 0;
+}
+
 // Everything the calling thread has issued to the tensor core so far arrives on bar when done.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -240,8 +257,9 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
 // A wait by a whole warp.  One that gives up sets the CTA's abort flag, which
 // ends every other wait; the warp's lanes leave together or not at all.  The
 // limit is a number of tries: reading the timer between them, or trying more
-// often, takes issue slots from the warps that are waited for (beams 614 k
-// cycles with the timer, 575 k without, 770 k with a spin of test_wait).
+// often, takes issue slots from the warps that are waited for (32 x 128 beams
+// behind 600 to 2600 keys: 614 k cycles with the timer, 575 k without, 770 k with
+// a spin of test_wait).
 constexpr int kTries = 500000;    // about 2 s: a try that fails sleeps some 4 us
 __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity) {
   for (int i = 0; i < kTries; ++i) {
@@ -251,6 +269,7 @@ __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity)
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
 }
+
 // ---------------------------------------------------------------- geometry
 struct Seq {          // a request
   int q0, n, len;     // first query token, query tokens, keys
@@ -333,13 +352,14 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t
 
 // The plan, by one CTA: the query blocks (request, block) in order, the exclusive
 // sums of their units, and the borders of the CTAs' runs.
-constexpr int kPlanItems = 2048;   // sums kept in shared memory for the search of the borders
+constexpr int kPlanItems = 1536;   // sums kept in shared memory for the search of the borders
 
 template <int BN>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int per, int max_items, int ctas) {
   __shared__ int64_t part[33];
   __shared__ int64_t s_pre[kPlanItems + 1];
   __shared__ int2 s_item[kPlanItems];
+  __shared__ int64_t s_first[kPlanThreads];
   __shared__ int64_t s_border[kMaxCtas + 1];
   gr::pdl_trigger();
   for (int i = threadIdx.x; i < ctas * 8; i += kPlanThreads) P.flag[i] = 0;
@@ -348,10 +368,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
   for (int r0 = 0; r0 < P.num_seqs; r0 += kPlanThreads) {
     const int r = r0 + static_cast<int>(threadIdx.x);
     const int nb = r < P.num_seqs ? blocks_of(load_seq(P, r, &bad), per) : 0;
-    const int64_t first = items + block_scan(nb, total, part);
-    for (int b = 0; b < nb && first + b < max_items; ++b) {
-      P.item[first + b] = make_int2(r, b);
-      if (first + b < kPlanItems) s_item[first + b] = make_int2(r, b);
+    s_first[threadIdx.x] = block_scan(nb, total, part);
+    __syncthreads();
+    // this pass's blocks, each by the last request that starts at or before it
+    for (int64_t i = threadIdx.x; i < total && items + i < max_items; i += kPlanThreads) {
+      int lo = 0, hi = kPlanThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_first[mid] <= i) lo = mid; else hi = mid - 1;
+      }
+      const int2 it = make_int2(r0 + lo, static_cast<int>(i - s_first[lo]));
+      P.item[items + i] = it;
+      if (items + i < kPlanItems) s_item[items + i] = it;
     }
     items += total;
   }
@@ -597,13 +625,12 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
 // Warp 1: the matrix products, issued by one lane.  The issue of a product holds
 // the warp about as long as the product takes, so whatever it does between two
 // batches is time that the tensor pipe stands still.  All control flow is by the
-// whole warp, so that operands are known to be uniform (3 to 6 % fewer cycles than
-// a role of one lane, 2048-key prompts and beams).
+// whole warp, so that operands are known to be uniform (2 to 6 % fewer cycles than
+// a role of one lane: a prompt of 8192, 32 x 128 beams).
 template <class S, bool kBf16>
 __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t data) {
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, sh->tmem, 0);
-  uint32_t leader;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(leader));
+  const bool leader = elect_lane();
   const auto commit = [&](uint64_t* bar) {
     if (leader) tc_commit(bar);
   };
@@ -870,7 +897,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u);
 }
 
-// Warps 4..: softmax of one query tile, one thread per row; also the rare
+// The last warps: softmax of one query tile, one thread per row; also the rare
 // rescaling of the accumulator, and the block's output.
 template <class S, bool kBf16>
 __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32_t data, int slot) {
@@ -1191,7 +1218,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     } else if (warp == 1) {
       mma_role<S, kBf16>(P, sh, base);
       if (*reinterpret_cast<volatile int*>(&sh->abort)) {   // products in flight finish before the tensor memory goes
-        if (lane == 0) tc_commit(&sh->drain);
+        if (elect_lane()) tc_commit(&sh->drain);
         __syncwarp();
         gr::mbar_wait_bounded(&sh->drain, 0);
       }
@@ -1252,8 +1279,8 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
   if (d->num_seqs < 0 || d->num_tokens < 0 || d->num_heads <= 0 || d->num_kv_heads <= 0 || d->head_dim <= 0 ||
       d->block_size <= 0 || d->max_blocks < 0 || d->num_blocks < 0 || d->num_blocks >= 0x7FFFFFFF ||
       d->num_heads % d->num_kv_heads != 0 || (d->causal != 0 && d->causal != 1) || d->max_query_len < 0 ||
-      !(d->scale > 0.0f) || d->scale > 3.0e38f || (d->num_seqs > 1 && d->table_stride < d->max_blocks) ||
-      static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7FFFFFFF - 256)
+      !(d->scale > 0.0f) || d->scale > 2.0e38f || (d->num_seqs > 1 && d->table_stride < d->max_blocks) ||
+      static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7FFFFFFF - 1024 || d->num_tokens > 0x7FFFFFFF - 1024)
     return GR_ERR_BAD_DESC;
   if (d->dtype != GR_DTYPE_BF16 && d->dtype != GR_DTYPE_F16) return GR_ERR_DTYPE;
   g.group = d->num_heads / d->num_kv_heads;
