@@ -499,7 +499,9 @@ typedef struct gr_paged_attn_io {
 } gr_paged_attn_io;
 
 /* Bytes of workspace gr_paged_attention() needs for `desc` (256-byte aligned,
- * contents need not be initialised; calls that share it must not overlap). */
+ * contents need not be initialised; calls that share it must not overlap).  A
+ * captured call that has set GR_DEVERR_TIMEOUT must be captured anew before it
+ * is replayed: the workspace may hold parts of the run that gave up. */
 int32_t gr_paged_attention_workspace_size(const gr_paged_attn_desc* desc, size_t* bytes);
 
 int32_t gr_paged_attention(const gr_paged_attn_desc* desc, const gr_paged_attn_io* io, void* workspace,

@@ -177,7 +177,7 @@ def test_long_caches_split_over_the_grid():
     b.check(*b.run(max_new=100))
 
 
-@pytest.mark.parametrize("R", [97, 1024, 1025, 2300])
+@pytest.mark.parametrize("R", [95, 96, 97, 1024, 1025, 2300])
 def test_many_requests(R):
     rng = np.random.default_rng(R)
     ctx, new = rng.integers(0, 90, R), rng.integers(0, 3, R)
@@ -423,7 +423,7 @@ def test_captured_beside_eager_calls_and_on_another_stream():
         for (_, res), want in zip(graphs, (want1, want2)):
             assert torch.equal(res[0], want[0]) and torch.equal(res[1], want[1])
         assert torch.equal(got[0], want1[0]) and torch.equal(got[1], want1[1])
-    # a replay reads new lengths: the second request shrinks
+    # a replay reads new lengths
     lens.copy_(_i32([701, 95, 1501]))
     graphs[0][0].replay()
     torch.cuda.synchronize()

@@ -18,7 +18,8 @@
 //
 // Work.  A (query block, KV head) pair of n key tiles costs n + kCost units; the
 // batch's units, in order, are cut into equal runs, one per CTA (one persistent
-// CTA per SM), whatever the lengths (plan_kernel, one CTA, ahead).  A border that
+// CTA per SM), whatever the lengths (planned by a one-CTA kernel ahead, or, up to
+// 96 query blocks, by every CTA for itself).  A border that
 // falls into a short pair moves to the pair's nearer end; a longer pair is cut.
 // The CTA with a cut pair's end owns it: the others leave partial outputs and
 // log-sums in the workspace, which the owner joins in run order.  Where whole
@@ -44,6 +45,8 @@
 // query tile (exponential unit and tensor pipe each near half of their rate), and
 // in long runs the power limit.
 
+#include <atomic>
+#include <chrono>
 #include <cstdint>
 #include <cstdlib>
 #include <cuda.h>
@@ -65,6 +68,7 @@ using gr::smem_u32;
 
 constexpr int kRows = 128;            // rows of a query tile (the matrix product's M)
 constexpr int kMaxCtas = 160;
+constexpr int kSmallItems = 96;       // requests and query blocks that the CTAs plan for themselves
 constexpr int kWorkRing = 4;          // (block, head) pairs handed out ahead
 // The shares of the work, in units of a key tile (about 2 us with two query tiles).  Measured on
 // 64 single tokens, a prompt of 8192, ragged chunks and beams: kCost 1 and 3, kMinRun 3 and 4,
@@ -121,6 +125,11 @@ struct Shared {
   uint64_t drain;
   uint32_t tmem;
   int abort;
+  // a small batch's plan: the runs' borders, the units before each query block, request and block
+  int64_t part[13];
+  int32_t border[kMaxCtas + 1], pre[kSmallItems + 1];
+  uint8_t req[kSmallItems], blk[kSmallItems];
+  int32_t items;
 };
 
 struct Run {                       // where a CTA's run starts
@@ -151,7 +160,9 @@ struct Params {
   int2* item;                      // request, block
   int32_t* items;                  // how many
   Run* run;                        // [ctas + 1]
-  int32_t* flag;                   // [ctas][2][4] part written (query tile, warp of it)
+  uint64_t* flag;                  // [ctas][2][4] part written (query tile, warp of it): token, until its owner has read it
+  uint64_t token;                  // of this call
+  int small;                       // planned by the CTAs
   float4* part_o;                  // [ctas][2][NQ][DP / 4][128 rows]: a warp's stores of its 32 rows are whole lines
   float* part_lse;                 // [ctas][2][NQ][128 rows]
 };
@@ -332,7 +343,8 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {
 
 constexpr int kPlanThreads = 1024;
 
-// Exclusive sum over a CTA of kPlanThreads; total in `total`.
+// Exclusive sum over a CTA of kT threads; total in `total`; part has kT / 32 + 1 places.
+template <int kT>
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t inc = warp_scan(v);
@@ -340,14 +352,51 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t
   if (lane == 31) part[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    const int64_t p = part[lane];
+    const int64_t p = lane < kT / 32 ? part[lane] : 0;
     const int64_t q = warp_scan(p);
-    part[lane] = q - p;
-    if (lane == 31) part[32] = q;
+    if (lane < kT / 32) part[lane] = q - p;
+    if (lane == 31) part[kT / 32] = q;
   }
   __syncthreads();
-  total = part[32];
+  total = part[kT / 32];
   return part[warp] + inc - v;
+}
+
+// Last index in [0, n) whose value is <= x (values ascending, v[0] <= x).
+template <typename T>
+__device__ __forceinline__ int last_le(const T* v, int n, int64_t x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (v[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Border c of `runs` runs over `all` units (`units` per KV head, `pre` before each of `items` query
+// blocks): at the even share (a short pair's nearer end), and at the nearer end of the pair that the
+// even share falls into.
+struct Border {
+  int64_t even, whole;
+  int64_t pair;        // first unit of that pair
+  int head, item;      // which it is
+};
+template <typename T>
+__device__ __forceinline__ Border border(const T* pre, int items, int64_t units, int64_t all, int64_t runs, int c) {
+  Border b{all, all, all, 0, items};
+  if (c >= runs) return b;
+  const int64_t u = all * c / runs;
+  b.head = static_cast<int>(u / units);
+  const int64_t in = u - b.head * units;
+  b.item = last_le(pre, items, in);
+  const int64_t span = pre[b.item + 1] - pre[b.item], off = in - pre[b.item];
+  b.pair = u - off;
+  b.whole = b.pair + (2 * off < span ? 0 : span);
+  b.even = span <= kSnap ? b.whole : u;
+  return b;
+}
+__device__ __forceinline__ int64_t runs_of(int64_t all, int ctas) {
+  return min(static_cast<int64_t>(ctas), max(all / kMinRun, static_cast<int64_t>(all > 0)));
 }
 
 // The plan, by one CTA: the query blocks (request, block) in order, the exclusive
@@ -362,21 +411,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
   __shared__ int64_t s_first[kPlanThreads];
   __shared__ int64_t s_border[kMaxCtas + 1];
   gr::pdl_trigger();
-  for (int i = threadIdx.x; i < ctas * 8; i += kPlanThreads) P.flag[i] = 0;
   int64_t items = 0, total;
   int bad = 0;
   for (int r0 = 0; r0 < P.num_seqs; r0 += kPlanThreads) {
     const int r = r0 + static_cast<int>(threadIdx.x);
     const int nb = r < P.num_seqs ? blocks_of(load_seq(P, r, &bad), per) : 0;
-    s_first[threadIdx.x] = block_scan(nb, total, part);
+    s_first[threadIdx.x] = block_scan<kPlanThreads>(nb, total, part);
     __syncthreads();
     // this pass's blocks, each by the last request that starts at or before it
     for (int64_t i = threadIdx.x; i < total && items + i < max_items; i += kPlanThreads) {
-      int lo = 0, hi = kPlanThreads - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_first[mid] <= i) lo = mid; else hi = mid - 1;
-      }
+      const int lo = last_le(s_first, kPlanThreads, i);
       const int2 it = make_int2(r0 + lo, static_cast<int>(i - s_first[lo]));
       P.item[items + i] = it;
       if (items + i < kPlanItems) s_item[items + i] = it;
@@ -395,7 +439,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
       const Seq s = load_seq(P, it.x);
       u = key_tiles<BN>(s, P.causal, it.y * per, min(s.n, (it.y + 1) * per)).n + kCost;
     }
-    const int64_t ex = block_scan(u, total, part);
+    const int64_t ex = block_scan<kPlanThreads>(u, total, part);
     if (i < items) {
       P.pre[i] = units + ex;
       if (i < kPlanItems) s_pre[i] = units + ex;
@@ -408,40 +452,63 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const Params P, int 
     if (items <= kPlanItems) s_pre[items] = units;
   }
   __syncthreads();
-  // border c at the even share, or at the nearer end of the pair that it falls into
   const int64_t* pre = items <= kPlanItems ? s_pre : P.pre;
-  const int64_t all = units * P.kv_heads;
-  const int64_t runs = items == 0 ? 0 : min(static_cast<int64_t>(ctas), max(all / kMinRun, static_cast<int64_t>(1)));
-  Run even{all, P.kv_heads - 1, static_cast<int>(items) - 1}, whole = even;
-  const int c = threadIdx.x;
-  if (c < runs) {
-    const int64_t u = all * c / runs;
-    const int head = static_cast<int>(u / units);
-    const int64_t in = u - head * units;
-    int lo = 0, hi = static_cast<int>(items) - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] <= in) lo = mid; else hi = mid - 1;
-    }
-    const int64_t span = pre[lo + 1] - pre[lo], off = in - pre[lo];
-    whole.u = u - off + (2 * off < span ? 0 : span);
-    even.u = span <= kSnap ? whole.u : u;
-    // the pair of the unit before the border
-    const auto before = [&](Run& r) {
-      const bool here = r.u > u - off;
-      r.head = here || lo > 0 ? head : head - 1;
-      r.item = here ? lo : (lo > 0 ? lo - 1 : static_cast<int>(items) - 1);
-    };
-    before(even);
-    before(whole);
-  }
+  const int64_t all = units * P.kv_heads, runs = runs_of(all, ctas);
+  const int c = threadIdx.x, n = static_cast<int>(items);
+  const Border at = border(pre, n, units, all, runs, c);
+  if (c <= ctas) s_border[c] = at.whole;
+  __syncthreads();
   // the longest run of whole pairs
-  __syncthreads();
-  if (c <= ctas) s_border[c] = whole.u;
-  __syncthreads();
   const bool longer = c < ctas && s_border[c + 1] - s_border[c] > all / max(runs, static_cast<int64_t>(1)) + kJoin;
   const bool cut = __syncthreads_or(longer);
-  if (c <= ctas) P.run[c] = cut ? even : whole;
+  if (c <= ctas) {
+    // with the pair of the unit before the border
+    Run r{cut ? at.even : at.whole, P.kv_heads - 1, n - 1};
+    if (c < runs && r.u > at.pair) {
+      r.head = at.head;
+      r.item = at.item;
+    } else if (c < runs) {
+      r.head = at.item > 0 ? at.head : at.head - 1;
+      r.item = at.item > 0 ? at.item - 1 : n - 1;
+    }
+    P.run[c] = r;
+  }
+}
+
+// The same for a small batch, by every CTA for itself in its shared memory: one
+// launch less, and the sums are a few hundred cycles.
+template <class S>
+__device__ __forceinline__ void plan_small(const Params& P, Shared* sh) {
+  const int tid = threadIdx.x, ctas = gridDim.x;
+  const int per = S::NQ * P.tp;
+  int64_t total;
+  int bad = 0;
+  const int nb = tid < P.num_seqs ? blocks_of(load_seq(P, tid, &bad), per) : 0;
+  const int64_t first = block_scan<S::kThreads>(nb, total, sh->part);
+  if (bad && blockIdx.x == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_RECORD);
+  const int items = static_cast<int>(min(total, static_cast<int64_t>(kSmallItems)));
+  if (tid <= P.num_seqs && tid <= kMaxCtas) sh->border[tid] = static_cast<int>(first);   // (for the search)
+  __syncthreads();
+  int64_t u = 0;
+  if (tid < items) {
+    const int r = last_le(sh->border, P.num_seqs, tid), b = tid - sh->border[r];
+    const Seq s = load_seq(P, r);
+    u = key_tiles<S::BN>(s, P.causal, b * per, min(s.n, (b + 1) * per)).n + kCost;
+    sh->req[tid] = static_cast<uint8_t>(r);
+    sh->blk[tid] = static_cast<uint8_t>(b);
+  }
+  int64_t units;
+  const int64_t before = block_scan<S::kThreads>(u, units, sh->part);
+  if (tid <= items) sh->pre[tid] = static_cast<int>(tid < items ? before : units);
+  if (tid == 0) sh->items = items;
+  __syncthreads();
+  const int64_t all = units * P.kv_heads, runs = runs_of(all, ctas);
+  const Border at = border(sh->pre, items, units, all, runs, tid);
+  if (tid <= ctas) sh->border[tid] = static_cast<int>(at.whole);
+  __syncthreads();
+  const bool longer =
+      tid < ctas && sh->border[tid + 1] - sh->border[tid] > all / max(runs, static_cast<int64_t>(1)) + kJoin;
+  if (__syncthreads_or(longer) && tid <= ctas) sh->border[tid] = static_cast<int>(at.even);
 }
 
 __device__ __forceinline__ int tile_at(const Work& k, int j) { return j < k.ta ? j : j - k.ta + k.tb; }
@@ -476,18 +543,31 @@ __device__ __forceinline__ bool next_work(Shared* sh, uint32_t& seq, Work& k) {
 template <class S>
 __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
   const int lane = threadIdx.x & 31;
-  const int64_t begin = P.run[blockIdx.x].u;
-  const Run stop = P.run[blockIdx.x + 1];
-  int64_t u = stop.u;
+  const auto run_at = [&](int c) { return P.small ? static_cast<int64_t>(sh->border[c]) : P.run[c].u; };
+  const int items = P.small ? sh->items : P.items[0];
+  const int64_t begin = run_at(blockIdx.x);
   const int per = S::NQ * P.tp;
+  int64_t u = run_at(blockIdx.x + 1);
+  // the pair of the run's last unit, and where that begins
+  int head, last;
+  int64_t beg;
+  if (P.small) {
+    const int units = sh->pre[items];
+    head = static_cast<int>((u - 1) / units);
+    last = last_le(sh->pre, items, u - 1 - static_cast<int64_t>(head) * units);
+    beg = static_cast<int64_t>(head) * units + sh->pre[last];
+  } else {
+    head = P.run[blockIdx.x + 1].head;
+    last = P.run[blockIdx.x + 1].item;
+    beg = head * P.pre[items] + P.pre[last];
+  }
   uint32_t seq = 0;
-  int64_t beg = u;                                   // of the pair; its last unit is the run's last one
-  for (int i = stop.item, head = stop.head; u > begin; --i) {
+  for (int i = last; u > begin; --i) {
     if (i < 0) {
       --head;
-      i = P.items[0] - 1;
+      i = items - 1;
     }
-    const int2 it = P.item[i];
+    const int2 it = P.small ? make_int2(sh->req[i], sh->blk[i]) : P.item[i];
     const Seq s = load_seq(P, it.x);
     Work k;
     k.req = it.x;
@@ -505,7 +585,7 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
     k.tb = t.b;
     k.n = t.n;
     const int span = t.n + kCost;
-    beg = seq == 0 && u == stop.u ? head * P.pre[P.items[0]] + P.pre[i] : u - span;
+    if (u <= beg) beg = u - span;                    // behind the first pair
     const int hi = static_cast<int>(u - beg);        // end of the run in the pair
     const int lo = static_cast<int>(max(begin - beg, static_cast<int64_t>(0)));
     k.j0 = max(lo - kCost, 0);
@@ -514,7 +594,7 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
     if (k.j1 <= k.j0) continue;
     k.part0 = blockIdx.x;
     if (k.j0 > 0 && k.j1 == k.n)                     // this CTA joins the parts
-      do --k.part0; while (k.part0 > 0 && P.run[k.part0].u > beg + kCost);
+      do --k.part0; while (k.part0 > 0 && run_at(k.part0) > beg + kCost);
     const int at = seq % kWorkRing;
     if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
     if (lane == 0) {
@@ -778,12 +858,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ void st_release(int32_t* p, int32_t v) {
-  asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ void st_release(uint64_t* p, uint64_t v) {
+  asm volatile("st.release.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
-__device__ __forceinline__ int32_t ld_acquire(const int32_t* p) {
-  int32_t v;
-  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+__device__ __forceinline__ uint64_t ld_acquire(const uint64_t* p) {
+  uint64_t v;
+  asm volatile("ld.acquire.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
 
@@ -821,12 +901,20 @@ __device__ __forceinline__ bool wait_parts(const Params& P, Shared* sh, int part
   bool ok = true;
   const uint64_t since = gr::global_timer_ns();
   for (int p = part0 + (threadIdx.x & 31); p < static_cast<int>(blockIdx.x); p += 32) {
-    while (ok && ld_acquire(P.flag + (p * 2 + slot) * 4 + warp) == 0)
+    while (ok && ld_acquire(P.flag + (p * 2 + slot) * 4 + warp) != P.token)
       ok = *reinterpret_cast<volatile int*>(&sh->abort) == 0 && gr::global_timer_ns() - since < gr::kWaitLimitNs;
   }
   if (__all_sync(0xFFFFFFFFu, ok)) return true;
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
+}
+
+// The parts are read: their flags go back to 0, so that a replay of this call, which has the same
+// token, waits again.
+__device__ __forceinline__ void free_parts(const Params& P, int part0, int slot, int warp) {
+  __syncwarp();
+  for (int p = part0 + (threadIdx.x & 31); p < static_cast<int>(blockIdx.x); p += 32)
+    P.flag[(p * 2 + slot) * 4 + warp] = 0;
 }
 
 // The join of a warp of at most 16 rows (single tokens, often cut over many
@@ -1153,9 +1241,10 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
         if (owner) {
           join_few<S, kBf16>(P, k, slot, warp, rows);
         } else if (lane == 0) {
-          st_release(P.flag + (blockIdx.x * 2 + slot) * 4 + warp, 1);
+          st_release(P.flag + (blockIdx.x * 2 + slot) * 4 + warp, P.token);
         }
       }
+      if (owner) free_parts(P, k.part0, slot, warp);
     } else {
       tc_fence_before();
       __syncwarp();
@@ -1202,8 +1291,15 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   __syncthreads();
   tc_fence_after();
 
-  gr::pdl_wait();      // the plan is complete
-  const bool busy = P.run[blockIdx.x].u < P.run[blockIdx.x + 1].u;
+  bool busy;
+  if (P.small) {
+    plan_small<S>(P, sh);
+    __syncthreads();
+    busy = sh->border[blockIdx.x] < sh->border[blockIdx.x + 1];
+  } else {
+    gr::pdl_wait();      // the plan is complete
+    busy = P.run[blockIdx.x].u < P.run[blockIdx.x + 1].u;
+  }
   // registers: 12 warps of 168 at launch give 4 x 56 + 8 x 224 (kNQ = 2), and 8 x 80 + 4 x 240 leave some (kNQ = 1)
   static_assert(S::kThreads == 384, "register split");
   if (warp < S::kSoftmax) {
@@ -1293,9 +1389,27 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
   g.box = 8;
   while (g.box * 2 <= g.bn && d->block_size % (g.box * 2) == 0) g.box *= 2;
   const int64_t per = static_cast<int64_t>(g.nq) * g.tp;
-  g.max_items = static_cast<int64_t>(d->num_tokens) / per + d->num_seqs;
+  // one more for each request with tokens than whole blocks
+  const int64_t some = d->num_seqs < d->num_tokens ? d->num_seqs : d->num_tokens;
+  g.max_items = static_cast<int64_t>(d->num_tokens) / per + some;
+  if (g.max_items > d->num_tokens) g.max_items = d->num_tokens;
   if (g.max_items > 0x7FFFFFFF) return GR_ERR_UNSUPPORTED;
   return GR_OK;
+}
+
+// Whether every CTA plans for itself: few query blocks, and units that fit 32 bits.
+static bool small_plan(const gr_paged_attn_desc* d, const Geometry& g) {
+  const int64_t tiles = static_cast<int64_t>(d->max_blocks) * d->block_size / 128 + 1 + kCost;
+  return d->num_seqs <= kSmallItems && g.max_items <= kSmallItems &&
+         tiles * kSmallItems * d->num_kv_heads < 0x7FFFFFFF;
+}
+
+// A number that no other call of this process has, and that stale memory holds by a chance of 2^-64.
+static uint64_t next_token() {
+  static std::atomic<uint64_t> next{static_cast<uint64_t>(std::chrono::steady_clock::now().time_since_epoch().count()) *
+                                        0x9E3779B97F4A7C15ull ^ reinterpret_cast<uintptr_t>(&g_attr)};
+  uint64_t t = next.fetch_add(0x9E3779B97F4A7C15ull, std::memory_order_relaxed);
+  return t != 0 ? t : next.fetch_add(0x9E3779B97F4A7C15ull, std::memory_order_relaxed);
 }
 
 static size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -1312,7 +1426,7 @@ static Layout layout(const gr_paged_attn_desc* d, const Geometry& g) {
     return here;
   };
   l.run = take(sizeof(Run) * (kMaxCtas + 1));
-  l.flag = take(sizeof(int32_t) * kMaxCtas * 8);
+  l.flag = take(sizeof(uint64_t) * kMaxCtas * 8);
   l.part_lse = take(sizeof(float) * kMaxCtas * 2 * g.nq * kRows);
   l.part_o = take(sizeof(float) * static_cast<size_t>(kMaxCtas) * 2 * g.nq * kRows * g.dp);
   l.pre = take(sizeof(int64_t) * (g.max_items + 1));
@@ -1362,10 +1476,11 @@ static int run(const Params& P, const Geometry& g, const CUtensorMap& mq, const 
     }
   }
   const int ctas = sms < kMaxCtas ? sms : kMaxCtas;
-  if (launch(plan_kernel<S::BN>, dim3(1), kPlanThreads, 0, s, false, P, S::NQ * P.tp, static_cast<int>(g.max_items),
+  if (!P.small &&
+      launch(plan_kernel<S::BN>, dim3(1), kPlanThreads, 0, s, false, P, S::NQ * P.tp, static_cast<int>(g.max_items),
              ctas) != cudaSuccess)
     return GR_ERR_CUDA;
-  if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, true, P, mq, mk, mv) != cudaSuccess)
+  if (launch(attention_kernel<S, kBf16>, dim3(ctas), S::kThreads, smem, s, !P.small, P, mq, mk, mv) != cudaSuccess)
     return GR_ERR_CUDA;
   return GR_OK;
 }
@@ -1455,7 +1570,9 @@ extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_page
   P.scale = d->scale;
   P.scale_log2 = d->scale * gr::kLog2e;
   P.run = reinterpret_cast<Run*>(ws + l.run);
-  P.flag = reinterpret_cast<int32_t*>(ws + l.flag);
+  P.flag = reinterpret_cast<uint64_t*>(ws + l.flag);
+  P.token = next_token();
+  P.small = small_plan(d, g);
   P.part_lse = reinterpret_cast<float*>(ws + l.part_lse);
   P.part_o = reinterpret_cast<float4*>(ws + l.part_o);
   P.pre = reinterpret_cast<int64_t*>(ws + l.pre);
