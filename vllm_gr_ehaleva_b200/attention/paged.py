@@ -34,13 +34,24 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurr
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(fn, name, index, *args):
-    """Calls an entry point on device `index`'s current stream, with the device current."""
+# torch.empty_strided on the current device without the argument parser (0.75 us instead of 1.3
+# to 2.3 us a tensor, a quarter of a small call), where this torch has it
+try:
+    _empty = torch._C._dynamo.guards._empty_strided_cuda
+except AttributeError:
+    def _empty(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+
+def _on(index, fn, *args):
+    """fn(*args) with device `index` current."""
     if index == torch.cuda.current_device():
-        rc = fn(*args, _stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _stream(index))
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _check(rc, name):
     if rc != _lib.GR_OK:
         raise RuntimeError(f"{name} failed: {_lib.STATUS_NAMES.get(rc, rc)}")
 
@@ -116,7 +127,7 @@ def _table_desc(block_table, cached_lens, new_lens, free_blocks, block_size, num
     _check_ints("new_lens", new_lens, device, _I32, (R,))
     _check_ints("free_blocks", free_blocks, device, _I32)
     d = _lib.BlockTableDesc(R, n, free_blocks.numel(), block_size, block_table.shape[1], 0, block_table.stride(0))
-    return d, R, n, device.index
+    return d, device.index
 
 
 def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_size: int, num_tokens: int, *, err=None):
@@ -139,17 +150,19 @@ def extend_block_tables(block_table, cached_lens, new_lens, free_blocks, block_s
            cached_lens.stride(), cached_lens.dtype, cached_lens.device, new_lens.shape, new_lens.stride(), new_lens.dtype,
            new_lens.device, free_blocks.shape, free_blocks.stride(), free_blocks.dtype, free_blocks.device, block_size,
            num_tokens)
-    d, R, n, index = _table_descs.get(key, _table_desc, block_table, cached_lens, new_lens, free_blocks, block_size,
-                                      num_tokens)
-    err = _err(err, block_table.device)
-    ints = block_table.new_empty(2 * R + 2)
-    longs = block_table.new_empty((2, n), dtype=_I64)
-    at, to = ints.data_ptr(), longs.data_ptr()
-    _call(_lib.load().gr_extend_block_tables, "gr_extend_block_tables", index, d, block_table.data_ptr(),
-          cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), at, at + 4 * (R + 1), to, to + 8 * n,
-          at + 4 * (2 * R + 1), err)
-    cu, lens, used = ints.split_with_sizes((R + 1, R, 1))
-    slots, positions = longs.unbind(0)
+    d, index = _table_descs.get(key, _table_desc, block_table, cached_lens, new_lens, free_blocks, block_size, num_tokens)
+    return _on(index, _extend, d, index, block_table, cached_lens, new_lens, free_blocks,
+               _err(err, block_table.device))
+
+
+def _extend(d, index, block_table, cached_lens, new_lens, free_blocks, err):
+    R, n = d.num_seqs, d.num_tokens
+    cu, lens, used = _empty((R + 1,), (1,), _I32), _empty((R,), (1,), _I32), _empty((1,), (1,), _I32)
+    slots, positions = _empty((n,), (1,), _I64), _empty((n,), (1,), _I64)
+    _check(_lib.load().gr_extend_block_tables(
+        d, block_table.data_ptr(), cached_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), cu.data_ptr(),
+        lens.data_ptr(), slots.data_ptr(), positions.data_ptr(), used.data_ptr(), err, _stream(index)),
+        "gr_extend_block_tables")
     return {"cu_seqlens_q": cu, "seq_lens": lens, "slot_mapping": slots, "positions": positions, "blocks_used": used}
 
 
@@ -189,8 +202,8 @@ def store_kv(k, v, k_cache, v_cache, slot_mapping, *, err=None) -> None:
     d, index, any_rows = _store_descs.get(key, _store_desc, k, v, k_cache, v_cache, slot_mapping)
     err = _err(err, k_cache.device)
     if any_rows:
-        _call(_lib.load().gr_store_kv, "gr_store_kv", index, d, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
-              v_cache.data_ptr(), slot_mapping.data_ptr(), err)
+        _check(_on(index, _lib.load().gr_store_kv, d, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                   slot_mapping.data_ptr(), err, _stream(index)), "gr_store_kv")
 
 
 def _attn_desc(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seqlen_q, scale, causal, beam_tail,
@@ -234,7 +247,7 @@ def _attn_desc(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seq
                            *k_cache.stride()[:3], *v_cache.stride()[:3], out_tok, out_head)
     size = ctypes.c_size_t(0)
     _lib.check(_lib.load().gr_paged_attention_workspace_size(d, size), "gr_paged_attention_workspace_size")
-    return d, size.value, device.index, bool(T and R)
+    return d, size.value, device.index, bool(T and R), ((T, H, D), (H * D, D, 1)), ((T, H), (H, 1))
 
 
 def _kind(t):
@@ -277,19 +290,24 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, ma
            block_table.dtype, block_table.device, cu_seqlens_q.shape, cu_seqlens_q.stride(), cu_seqlens_q.dtype,
            cu_seqlens_q.device, seq_lens.shape, seq_lens.stride(), seq_lens.dtype, seq_lens.device, max_seqlen_q, scale,
            causal, _kind(beam_tail), _kind(beam_steps), _kind(out))
-    d, size, index, any_rows = _attn_descs.get(key, _attn_desc, q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens,
-                                               max_seqlen_q, scale, causal, beam_tail, beam_steps, out)
-    err = _err(err, q.device)
+    desc = _attn_descs.get(key, _attn_desc, q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seqlen_q, scale,
+                           causal, beam_tail, beam_steps, out)
+    return _on(desc[2], _attend, desc, q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, beam_tail, beam_steps, out,
+               return_lse, _err(err, q.device))
+
+
+def _attend(desc, q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, beam_tail, beam_steps, out, return_lse, err):
+    d, size, index, any_rows, out_as, lse_as = desc
     if out is None:
-        out = q.new_empty(q.shape)
-    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+        out = _empty(*out_as, q.dtype)
+    lse = _empty(*lse_as, torch.float32) if return_lse else None
     if any_rows:
         # from the caching allocator per call: stream ordered, and a captured graph keeps its own
-        ws = q.new_empty(size, dtype=torch.uint8)
+        ws = _empty((size,), (1,), torch.uint8)
         io = _lib.PagedAttnIO(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
                               cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
                               None if beam_tail is None else beam_tail.data_ptr(),
                               None if beam_steps is None else beam_steps.data_ptr(), out.data_ptr(),
                               None if lse is None else lse.data_ptr(), err)
-        _call(_lib.load().gr_paged_attention, "gr_paged_attention", index, d, io, ws.data_ptr(), size)
+        _check(_lib.load().gr_paged_attention(d, io, ws.data_ptr(), size, _stream(index)), "gr_paged_attention")
     return (out, lse) if return_lse else out
