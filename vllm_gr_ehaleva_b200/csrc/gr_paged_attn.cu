@@ -271,9 +271,10 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
 // often, takes issue slots from the warps that are waited for (32 x 128 beams
 // behind 600 to 2600 keys: 614 k cycles with the timer, 575 k without, 770 k with
 // a spin of test_wait).
-constexpr int kTries = 500000;    // about 2 s: a try that fails sleeps some 4 us
-__device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity) {
-  for (int i = 0; i < kTries; ++i) {
+constexpr int kTries = 500000;           // about 2 s: a try that fails sleeps some 4 us
+constexpr int kPairTries = 16 * kTries;  // for waits that last as long as a pair does
+__device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity, int tries = kTries) {
+  for (int i = 0; i < tries; ++i) {
     if (__all_sync(0xFFFFFFFFu, gr::mbar_try_wait(bar, parity))) return true;
     if (*reinterpret_cast<volatile int*>(&sh->abort)) break;
   }
@@ -529,7 +530,7 @@ struct Ring {        // position in the ring of key and value tiles
 // The next (block, head) of the run; false at its end or when a wait gave up.
 __device__ __forceinline__ bool next_work(Shared* sh, uint32_t& seq, Work& k) {
   const int at = seq % kWorkRing;
-  if (!wait(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u)) return false;
+  if (!wait(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u, kPairTries)) return false;
   k = sh->work[at];
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->wk_empty[at]);
@@ -596,7 +597,7 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
     if (k.j0 > 0 && k.j1 == k.n)                     // this CTA joins the parts
       do --k.part0; while (k.part0 > 0 && run_at(k.part0) > beg + kCost);
     const int at = seq % kWorkRing;
-    if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
+    if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u, kPairTries)) return;
     if (lane == 0) {
       sh->work[at] = k;
       mbar_arrive(&sh->wk_full[at]);
@@ -604,7 +605,7 @@ __device__ __forceinline__ void schedule_role(const Params& P, Shared* sh) {
     ++seq;
   }
   const int at = seq % kWorkRing;
-  if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u)) return;
+  if (!wait(sh, &sh->wk_empty[at], ((seq / kWorkRing) & 1u) ^ 1u, kPairTries)) return;
   if (lane == 0) {
     sh->work[at].slots = 0;
     mbar_arrive(&sh->wk_full[at]);
@@ -632,7 +633,7 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
   int bad = 0;
   while (ok && next_work(sh, seq, k)) {
     if (kKeys && part == 0) {
-      if (!wait(sh, &sh->q_empty, qphase ^ 1u)) break;
+      if (!wait(sh, &sh->q_empty, qphase ^ 1u, kPairTries)) break;
       if (lane == 0 && !(P.flags & 1)) {
         const int slots = S::NQ == 2 ? k.slots : 1;
         mbar_arrive_expect_tx(&sh->q_full, static_cast<uint32_t>(slots * S::CH * P.group * P.tp * 128));
@@ -767,7 +768,7 @@ __device__ __forceinline__ void mma_role(const Params& P, Shared* sh, uint32_t d
   };
   for (uint32_t seq = 0;; ++seq) {
     const int at = seq % kWorkRing;
-    if (!wait(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u)) return;
+    if (!wait(sh, &sh->wk_full[at], (seq / kWorkRing) & 1u, kPairTries)) return;
     const int slots = __shfl_sync(0xFFFFFFFFu, sh->work[at].slots, 0);
     const int n = __shfl_sync(0xFFFFFFFFu, sh->work[at].j1 - sh->work[at].j0, 0);
     if (leader) mbar_arrive(&sh->wk_empty[at]);
@@ -895,14 +896,14 @@ __device__ __forceinline__ int64_t part_at(int p, int slot) {
   return (static_cast<int64_t>(p) * 2 + 1) * S::NQ + slot;
 }
 
-// Waits (bounded) until the CTAs from part0 up to this one have left this warp's
-// rows of their parts.
+// Waits (bounded; runs of many seconds may end some seconds apart) until the CTAs
+// from part0 up to this one have left this warp's rows of their parts.
 __device__ __forceinline__ bool wait_parts(const Params& P, Shared* sh, int part0, int slot, int warp) {
   bool ok = true;
   const uint64_t since = gr::global_timer_ns();
   for (int p = part0 + (threadIdx.x & 31); p < static_cast<int>(blockIdx.x); p += 32) {
     while (ok && ld_acquire(P.flag + (p * 2 + slot) * 4 + warp) != P.token)
-      ok = *reinterpret_cast<volatile int*>(&sh->abort) == 0 && gr::global_timer_ns() - since < gr::kWaitLimitNs;
+      ok = *reinterpret_cast<volatile int*>(&sh->abort) == 0 && gr::global_timer_ns() - since < 10 * gr::kWaitLimitNs;
   }
   if (__all_sync(0xFFFFFFFFu, ok)) return true;
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
