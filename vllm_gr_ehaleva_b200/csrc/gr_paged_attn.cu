@@ -918,42 +918,47 @@ __device__ __forceinline__ void free_parts(const Params& P, int part0, int slot,
     P.flag[(p * 2 + slot) * 4 + warp] = 0;
 }
 
-// The join of a warp of at most 16 rows (single tokens, often cut over many
-// CTAs): two or four lanes a row, this CTA's part read back from its place 0.
-template <class S, bool kBf16>
+// The join of a warp of at most 32 / kEach rows (single tokens, often cut over
+// many CTAs): kEach lanes a row, this CTA's part read back from its place 0, and as
+// many parts in flight as 32 vectors per lane allow.
+template <class S, bool kBf16, int kEach>
 __device__ __forceinline__ void join_few(const Params& P, const Work& k, int slot, int warp, int rows) {
-  constexpr int DP = S::DP;
+  constexpr int kVecs = S::DP / 4 / kEach < 8 ? S::DP / 4 / kEach : 8;   // a lane's vectors of a part at a time
+  constexpr int kAhead = 32 / kVecs;
   const int lane = threadIdx.x & 31;
   const int cta = blockIdx.x, parts = cta - k.part0 + 1;
-  const int each = rows <= 8 ? 4 : 2;   // lanes per row
-  const int r = lane % (32 / each), q = lane / (32 / each);
+  const int r = lane % (32 / kEach), q = lane / (32 / kEach);
   const int m_row = warp * 32 + min(r, rows - 1);
   const auto place = [&](int i) {
     const int p = k.part0 + i;
     return p == cta ? static_cast<int64_t>(p) * 2 * S::NQ + slot : part_at<S>(p, slot);
   };
   float top = -kInf;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(P.part_lse + place(i) * kRows + m_row));
+#pragma unroll 4
+  for (int i = q; i < parts; i += kEach) top = fmaxf(top, __ldcg(P.part_lse + place(i) * kRows + m_row));
+#pragma unroll
+  for (int o = 32 / kEach; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   const float ref = top == -kInf ? 0.0f : top;
   const int ti = m_row / P.group, g = m_row - ti * P.group;
   const int64_t t = static_cast<int64_t>(k.q0) + k.t0 + slot * P.tp + ti;
   const int h = k.kvh * P.group + g;
   unsigned char* orow = static_cast<unsigned char*>(P.out) + (t * P.out_tok + h * P.out_head) * 2;
-  constexpr int kAhead = 4;
-  for (int x = q * 32; x < DP; x += each * 32) {
-    float4 acc[8];
+#pragma unroll 1
+  for (int x = q * kVecs * 4; x < S::DP; x += kEach * kVecs * 4) {
+    float4 acc[kVecs];
 #pragma unroll
-    for (int y = 0; y < 8; ++y) acc[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int y = 0; y < kVecs; ++y) acc[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float sum = 0.0f;
+#pragma unroll 1
     for (int i = 0; i < parts; i += kAhead) {
-      float4 v[kAhead][8];
+      float4 v[kAhead][kVecs];
       float w[kAhead];
 #pragma unroll
       for (int z = 0; z < kAhead; ++z) {
         const int64_t at = place(min(i + z, parts - 1));
         w[z] = i + z < parts ? __ldcg(P.part_lse + at * kRows + m_row) : -kInf;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) v[z][y] = __ldcg(P.part_o + (at * (DP / 4) + x / 4 + y) * kRows + m_row);
+        for (int y = 0; y < kVecs; ++y) v[z][y] = __ldcg(P.part_o + (at * (S::DP / 4) + x / 4 + y) * kRows + m_row);
       }
 #pragma unroll
       for (int z = 0; z < kAhead; ++z) {
@@ -961,7 +966,7 @@ __device__ __forceinline__ void join_few(const Params& P, const Work& k, int slo
         const float wz = gr::fast_exp2(w[z] - ref);
         sum += wz;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
+        for (int y = 0; y < kVecs; ++y) {
           acc[y].x += wz * v[z][y].x;
           acc[y].y += wz * v[z][y].y;
           acc[y].z += wz * v[z][y].z;
@@ -970,11 +975,16 @@ __device__ __forceinline__ void join_few(const Params& P, const Work& k, int slo
       }
     }
     const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int y = 0; y < 8; ++y)
-      acc[y] = make_float4(acc[y].x * inv, acc[y].y * inv, acc[y].z * inv, acc[y].w * inv);
     if (r < rows) {
-      store32<kBf16>(P, orow, x, acc);
+#pragma unroll
+      for (int y = 0; y < kVecs; y += 2) {
+        const int col = x + y * 4;
+        if (col < P.dim)
+          *reinterpret_cast<uint4*>(orow + col * 2) =
+              make_uint4(pack16<kBf16>(acc[y].x * inv, acc[y].y * inv), pack16<kBf16>(acc[y].z * inv, acc[y].w * inv),
+                         pack16<kBf16>(acc[y + 1].x * inv, acc[y + 1].y * inv),
+                         pack16<kBf16>(acc[y + 1].z * inv, acc[y + 1].w * inv));
+      }
       if (x == 0 && P.lse)
         P.lse[t * P.heads + h] = sum > 0.0f || sum != sum ? (ref + __log2f(sum)) * kLn2 : -kInf;
     }
@@ -1028,7 +1038,6 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
       if (any_live) {
         const uint32_t s_col = tmem + b * BN;
         uint32_t sr[BN / 32][32], p[BN / 2];
-        const auto score = [&](int x) { return __uint_as_float(sr[x / 32][x % 32]); };
         const auto load = [&] {   // the tile's scores, -inf where the row does not see the key
 #pragma unroll
           for (int x = 0; x < BN / 32; ++x) tc_ld32(sr[x], s_col + x * 32);
@@ -1046,6 +1055,7 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
             }
           }
         };
+        const auto score = [&](int x) { return __uint_as_float(sr[x / 32][x % 32]); };
         const auto maximum = [&] {
           float t[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
@@ -1237,10 +1247,14 @@ __device__ __forceinline__ void softmax_role(const Params& P, Shared* sh, uint32
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->o_free[slot]);
       if (!done) {
-        __threadfence();
-        __syncwarp();
+        __syncwarp();   // orders the lanes' stores before lane 0's release, and before the reads of the join
         if (owner) {
-          join_few<S, kBf16>(P, k, slot, warp, rows);
+          if (rows <= 4)
+            join_few<S, kBf16, 8>(P, k, slot, warp, rows);
+          else if (rows <= 8)
+            join_few<S, kBf16, 4>(P, k, slot, warp, rows);
+          else
+            join_few<S, kBf16, 2>(P, k, slot, warp, rows);
         } else if (lane == 0) {
           st_release(P.flag + (blockIdx.x * 2 + slot) * 4 + warp, P.token);
         }
@@ -1261,7 +1275,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   Shared* sh = reinterpret_cast<Shared*>(raw + (base - smem_u32(raw)) + S::kData);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&sh->full[i], 1);
