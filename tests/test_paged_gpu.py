@@ -384,7 +384,7 @@ def test_refusals():
         with pytest.raises(ValueError, match=match):
             store_kv(*args)
     for match, args in (("rows for", (t, lens[:1], lens[:1], lens, 16, 3)), ("shape", (t, lens, lens[:1], lens, 16, 3)),
-                        ("int32", (t, lens, lens, lens.long(), 16, 3)), ("positive", (t, lens, lens, lens, 0, 3)),
+                        ("int32", (t, lens, lens, lens.long(), 16, 3)), ("positive", (t, lens, lens, lens, 0, 3)), ("2\\^31", (t, lens, lens, lens, 2 ** 32 + 16, 3)),
                         ("num_tokens", (t, lens, lens, lens, 16, -1)), ("1-D", (t, lens[None], lens, lens, 16, 3)),
                         ("overlap", (torch.zeros(4, dtype=torch.int32, device=DEV).as_strided((2, 3), (1, 1)), lens, lens, lens, 16, 3))):
         with pytest.raises(ValueError, match=match):

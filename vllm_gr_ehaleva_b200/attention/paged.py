@@ -84,6 +84,12 @@ def _check_caches(k_cache, v_cache):
         raise ValueError("k_cache and v_cache must have the same dtype, shape and device")
 
 
+def _check_sizes(*sizes):
+    """The library's descriptors hold these in 32 bits."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ValueError(f"sizes must be below 2^31, not {max(sizes)}")
+
+
 def _err(err, device):
     if err is None:
         return None
@@ -126,6 +132,7 @@ def _table_desc(block_table, cached_lens, new_lens, free_blocks, block_size, num
     _check_ints("cached_lens", cached_lens, device, _I32, (R,))
     _check_ints("new_lens", new_lens, device, _I32, (R,))
     _check_ints("free_blocks", free_blocks, device, _I32)
+    _check_sizes(R, free_blocks.numel(), block_size, block_table.shape[1])
     d = _lib.BlockTableDesc(R, n, free_blocks.numel(), block_size, block_table.shape[1], 0, block_table.stride(0))
     return d, device.index
 
@@ -182,6 +189,7 @@ def _store_desc(k, v, k_cache, v_cache, slot_mapping):
     if k.numel() and not k_cache.numel():
         raise ValueError("the cache has no blocks")
     nb, bs, heads, dim = k_cache.shape
+    _check_sizes(bs, heads, dim)
     d = _lib.KvStoreDesc(T, nb, bs, heads, dim, k_cache.element_size(), *k.stride(), *v.stride(), *k_cache.stride(),
                          *v_cache.stride())
     return d, device.index, k.numel() > 0
@@ -241,6 +249,7 @@ def _attn_desc(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, max_seq
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or
                             (D > 1 and out.stride(2) != 1)):
         raise ValueError("out must have q's shape, dtype and device and unit stride in head_dim")
+    _check_sizes(R, T, H, D, bs, block_table.shape[1])
     out_tok, out_head = (H * D, D) if out is None else out.stride()[:2]
     d = _lib.PagedAttnDesc(R, T, H, HK, D, bs, block_table.shape[1], _DTYPES[q.dtype], int(causal),
                            max_seqlen_q, scale, 0, nb, block_table.stride(0), q.stride(0), q.stride(1),
