@@ -415,6 +415,7 @@ int32_t gr_extend_block_tables(const gr_block_table_desc* desc, int32_t* block_t
  * [0, num_blocks * block_size) are skipped and set GR_DEVERR_BAD_SLOT in *err
  * (err may be NULL).  The slots of one call must differ from one another: of two
  * rows for one slot an unspecified mix may remain.  Strides are in elements.
+ * num_heads * head_dim at most 2^31 - 1024 (GR_ERR_BAD_DESC).
  * Replaces vLLM's reshape_and_cache_flash as the reference calls it
  * (beam_attn.py:727-732). */
 typedef struct gr_kv_store_desc {

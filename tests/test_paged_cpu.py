@@ -140,6 +140,17 @@ def test_block_table_and_store_arguments():
         assert store(ptrs=[None if j == i else 4096 for j in range(5)]) == NULL
 
 
+def test_store_refuses_rows_whose_indexes_pass_32_bits():
+    # a warp's element index runs up to 31 behind the row
+    def status(heads, dim):
+        d = _lib.KvStoreDesc(1, 2, 16, heads, dim, 1, *[1] * 14)
+        return _lib.load().gr_store_kv(d, None, *(4096,) * 4, None, None)
+
+    for heads, dim in ((1, 2 ** 31 - 1), (2 ** 31 - 1, 1), (2, 2 ** 30), (1, 2 ** 31 - 1023)):
+        assert status(heads, dim) == BAD, (heads, dim)
+    assert status(1, 2 ** 31 - 1024) == NULL   # the limit itself gets as far as the missing pointer
+
+
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
