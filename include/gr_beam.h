@@ -388,6 +388,7 @@ int32_t gr_remux_logprobs(const gr_remux_desc* desc, const int32_t* row_w, const
  * bits, and tokens beyond num_tokens give GR_DEVERR_BAD_RECORD: such a length
  * pair counts as no new token (a negative cached as 0), such tokens have no
  * entry.  err may be NULL; bits are OR-ed into it.  positions may be NULL.
+ * num_seqs at most 2^31 - 4096 (GR_ERR_BAD_DESC).
  * The reference leaves this to vLLM's host code (v1/worker/block_table.py,
  * NumPy loops and copies per step); its builder consumes the result
  * (beam_attn.py:432-476). */

@@ -151,6 +151,17 @@ def test_store_refuses_rows_whose_indexes_pass_32_bits():
     assert status(1, 2 ** 31 - 1024) == NULL   # the limit itself gets as far as the missing pointer
 
 
+def test_block_tables_refuse_batches_whose_indexes_pass_32_bits():
+    # the request index runs up to 2047 behind the batch
+    def status(num_seqs):
+        d = _lib.BlockTableDesc(num_seqs, 3, 4, 16, 5, 0, 5)
+        return _lib.load().gr_extend_block_tables(d, *[4096] * 4, None, *[4096] * 5, None)
+
+    for n in (2 ** 31 - 1, 2 ** 31 - 2048, 2 ** 31 - 4095):
+        assert status(n) == BAD, n
+    assert status(2 ** 31 - 4096) == NULL      # the limit itself gets as far as the missing pointer
+
+
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)

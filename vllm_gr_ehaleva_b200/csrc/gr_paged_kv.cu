@@ -322,7 +322,7 @@ extern "C" int32_t gr_extend_block_tables(const gr_block_table_desc* d, int32_t*
   using namespace grpk;
   if (!d) return GR_ERR_NULL;
   if (d->num_seqs < 0 || d->num_tokens < 0 || d->num_free < 0 || d->block_size < 1 || d->max_blocks < 0 ||
-      (d->num_seqs > 1 && d->table_stride < d->max_blocks))
+      d->num_seqs > 0x7FFFFFFF - 4095 || (d->num_seqs > 1 && d->table_stride < d->max_blocks))
     return GR_ERR_BAD_DESC;
   if (!cu_seqlens || !blocks_used) return GR_ERR_NULL;
   if (d->num_seqs > 0 && (!cached || !fresh || !seq_lens || (d->max_blocks > 0 && !block_table))) return GR_ERR_NULL;
