@@ -458,7 +458,7 @@ int32_t gr_store_kv(const gr_kv_store_desc* desc, const void* k, const void* v, 
  * the paged attention kernel (beam_attn.py:734-755).
  *
  * Limits (GR_ERR_UNSUPPORTED): head_dim a multiple of 8 up to 256; block_size a
- * multiple of 8; num_heads / num_kv_heads at most 128.  num_tokens and max_blocks *
+ * multiple of 8; num_heads / num_kv_heads at most 128.  num_seqs, num_tokens and max_blocks *
  * block_size at most 2^31 - 1024, num_blocks below 2^31 - 1 (GR_ERR_BAD_DESC).  Strides are in elements;
  * rows are contiguous in the head dimension, and every other stride and address
  * of q, the caches and out must be a multiple of 16 bytes (GR_ERR_MISALIGNED).

@@ -162,6 +162,14 @@ def test_block_tables_refuse_batches_whose_indexes_pass_32_bits():
     assert status(2 ** 31 - 4096) == NULL      # the limit itself gets as far as the missing pointer
 
 
+def test_attention_refuses_batches_whose_indexes_pass_32_bits():
+    # the request index runs up to 1023 behind the batch
+    n = ctypes.c_size_t(0)
+    for r in (2 ** 31 - 1, 2 ** 31 - 1023):
+        assert _lib.load().gr_paged_attention_workspace_size(_attn(num_seqs=r), n) == BAD, r
+    assert _lib.load().gr_paged_attention_workspace_size(_attn(num_seqs=2 ** 31 - 1024), n) == 0
+
+
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
