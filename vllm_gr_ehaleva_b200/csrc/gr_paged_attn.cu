@@ -1391,8 +1391,8 @@ static int geometry(const gr_paged_attn_desc* d, Geometry& g) {
       d->block_size <= 0 || d->max_blocks < 0 || d->num_blocks < 0 || d->num_blocks >= 0x7FFFFFFF ||
       d->num_heads % d->num_kv_heads != 0 || (d->causal != 0 && d->causal != 1) || d->max_query_len < 0 ||
       !(d->scale > 0.0f) || d->scale > 2.0e38f || (d->num_seqs > 1 && d->table_stride < d->max_blocks) ||
-      static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7FFFFFFF - 1024 ||
-      d->num_tokens > 0x7FFFFFFF - 1024 || d->num_seqs > 0x7FFFFFFF - 1023)
+      static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7FFFFFFF - 1023 ||
+      d->num_tokens > 0x7FFFFFFF - 1023 || d->num_seqs > 0x7FFFFFFF - 1023)
     return GR_ERR_BAD_DESC;
   if (d->dtype != GR_DTYPE_BF16 && d->dtype != GR_DTYPE_F16) return GR_ERR_DTYPE;
   g.group = d->num_heads / d->num_kv_heads;

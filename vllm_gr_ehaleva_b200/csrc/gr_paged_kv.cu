@@ -366,7 +366,7 @@ extern "C" int32_t gr_store_kv(const gr_kv_store_desc* d, const void* k, const v
   using namespace grpk;
   if (!d) return GR_ERR_NULL;
   if (d->num_tokens < 0 || d->num_blocks < 0 || d->block_size < 1 || d->num_heads <= 0 || d->head_dim <= 0 ||
-      static_cast<int64_t>(d->num_heads) * d->head_dim > 0x7FFFFFFF - 1024)
+      static_cast<int64_t>(d->num_heads) * d->head_dim > 0x7FFFFFFF - 1023)
     return GR_ERR_BAD_DESC;
   if (d->elem_bytes != 1 && d->elem_bytes != 2 && d->elem_bytes != 4) return GR_ERR_DTYPE;
   if (d->num_tokens == 0) return GR_OK;
