@@ -526,6 +526,26 @@ def test_block_tables_report_what_does_not_fit():
     assert (m["slot_mapping"] == -1).all() and int(m["cu_seqlens_q"]) == 0 and int(m["blocks_used"]) == 0
 
 
+@pytest.mark.parametrize("R", [3, 300])
+@pytest.mark.parametrize("bs", [1, 16])
+def test_block_tables_end_with_the_free_list_whatever_the_lengths_ask_for(R, bs):
+    # lengths near 2^31 ask for up to 10^11 blocks; the work is that of the 40 there are
+    free = np.random.default_rng(R).permutation(500).astype(np.int32)[:40]
+    table = torch.full((R, 50), -1, dtype=torch.int32, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    n = 41 * bs
+    m = extend_block_tables(table, _i32([0] * R), _i32([2 ** 31 - 1] * R), _i32(free), bs, n, err=err)
+    assert int(err) == 0x80 | 0x40
+    want = np.full((R, 50), -1, np.int32)
+    want[0, :40] = free
+    assert np.array_equal(table.cpu().numpy(), want)
+    assert (m["seq_lens"] == 2 ** 31 - 1).all() and int(m["blocks_used"]) == min(2 ** 31 - 1, R * -(-(2 ** 31 - 1) // bs))
+    assert m["cu_seqlens_q"].tolist() == [0] + [2 ** 31 - 1] * R
+    slots = np.concatenate([free.astype(np.int64).repeat(bs) * bs + np.tile(np.arange(bs), 40), np.full(bs, -1)])
+    assert np.array_equal(m["slot_mapping"].cpu().numpy(), slots)
+    assert m["positions"].tolist() == list(range(n))
+
+
 # ---------------------------------------------------------------- cache write
 @pytest.mark.parametrize("dtype", [BF16, F16, torch.float32, torch.uint8])
 @pytest.mark.parametrize("H,D,bs", [(8, 128, 16), (2, 256, 32), (1, 8, 1), (3, 5, 7), (1, 1, 16), (16, 256, 16)])

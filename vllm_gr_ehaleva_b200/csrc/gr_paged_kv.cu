@@ -149,12 +149,15 @@ __global__ void __launch_bounds__(kThreads) extend_block_tables_kernel(const Tab
       P.cu[r0 + r] = clamp32(s_cu[r]);
       P.seq_lens[r0 + r] = s_cached[r] + static_cast<int>(s_cu[r + 1] - s_cu[r]);
     }
-    // fresh blocks: entry e of the free list to its place in the table
-    const int64_t eb = blk0 + tb * me / G, ee = blk0 + tb * (me + 1) / G;
+    // fresh blocks: entry e of the free list to its place in the table.  The loop ends with the
+    // list, whatever the lengths ask for: lengths near 2^31 would make it 10^10 blocks.
+    const int64_t tf = min(tb, max(static_cast<int64_t>(P.num_free) - blk0, static_cast<int64_t>(0)));
+    if (tf < tb && me == 0 && threadIdx.x == 0) bad |= GR_DEVERR_NO_BLOCK;
+    const int64_t eb = blk0 + tf * me / G, ee = blk0 + tf * (me + 1) / G;
     for (int64_t e = eb + threadIdx.x; e < ee; e += kThreads) {
       const int r = last_le(s_base, nr, e);
       const int64_t j = blocks_of(s_cached[r], bs) + (e - s_base[r]);
-      if (e < P.num_free && j < P.max_blocks)
+      if (j < P.max_blocks)
         P.table[(r0 + r) * P.table_stride + j] = P.free_blocks[e];
       else
         bad |= GR_DEVERR_NO_BLOCK;
