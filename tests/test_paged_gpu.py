@@ -447,6 +447,23 @@ def test_expired_waits_report_and_return(monkeypatch):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_expired_waits_of_cut_pairs(monkeypatch):
+    # every CTA has a part of a pair: roles that wait for copies, for one another and for other
+    # CTAs' parts all leave; with few query blocks, and with a plan of its own kernel
+    for ctx, new in (([20000], [1]), ([20000] + [5] * 119, [1] * 120)):
+        b = Batch(ctx, new, 8, 2, 128, 16, BF16, seed=29)
+        want = b.run()
+        torch.cuda.synchronize()
+        monkeypatch.setenv("GR_TEST_STALL_COPIES", "1")
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        b.run(err=err)
+        torch.cuda.synchronize()
+        assert int(err) & 0x4
+        monkeypatch.delenv("GR_TEST_STALL_COPIES")
+        got = b.run()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 # ---------------------------------------------------------------- block tables and slot maps
 @pytest.mark.parametrize("R,bs", [(1, 16), (5, 1), (37, 16), (256, 16), (257, 16), (1024, 32), (2047, 16), (2048, 32), (2049, 48), (5000, 16)])
 def test_block_tables(R, bs):

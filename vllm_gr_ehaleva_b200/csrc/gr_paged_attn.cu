@@ -266,17 +266,22 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
 }
 
 // A wait by a whole warp.  One that gives up sets the CTA's abort flag, which
-// ends every other wait; the warp's lanes leave together or not at all.  The
+// ends every other wait; the warp's lanes leave together or not at all: they vote
+// on the flag too, since lanes that read it apart may read it differently, and one
+// that stayed would vote with lanes that have left.  The
 // limit is a number of tries: reading the timer between them, or trying more
 // often, takes issue slots from the warps that are waited for (32 x 128 beams
 // behind 600 to 2600 keys: 614 k cycles with the timer, 575 k without, 770 k with
 // a spin of test_wait).
 constexpr int kTries = 500000;           // about 2 s: a try that fails sleeps some 4 us
 constexpr int kPairTries = 16 * kTries;  // for waits that last as long as a pair does
+__device__ __forceinline__ bool aborted(Shared* sh) {   // one answer for the warp
+  return __any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile int*>(&sh->abort));
+}
 __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t parity, int tries = kTries) {
   for (int i = 0; i < tries; ++i) {
     if (__all_sync(0xFFFFFFFFu, gr::mbar_try_wait(bar, parity))) return true;
-    if (*reinterpret_cast<volatile int*>(&sh->abort)) break;
+    if (aborted(sh)) break;
   }
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
@@ -689,7 +694,7 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
     }
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_SLOT);
-  if (*reinterpret_cast<volatile int*>(&sh->abort)) {
+  if (aborted(sh)) {
     // gave up: wait (bounded) for this warp's copies in flight before the shared memory goes
     for (int i = 0; i < S::kStages; ++i) {
       if (ring.stage == 0) {
@@ -1328,7 +1333,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       schedule_role<S>(P, sh);
     } else if (warp == 1) {
       mma_role<S, kBf16>(P, sh, base);
-      if (*reinterpret_cast<volatile int*>(&sh->abort)) {   // products in flight finish before the tensor memory goes
+      if (aborted(sh)) {   // products in flight finish before the tensor memory goes
         if (elect_lane()) tc_commit(&sh->drain);
         __syncwarp();
         gr::mbar_wait_bounded(&sh->drain, 0);
