@@ -177,6 +177,19 @@ def test_long_caches_split_over_the_grid():
     b.check(*b.run(max_new=100))
 
 
+@pytest.mark.parametrize("D,dtype", [(128, BF16), (256, F16)])
+@pytest.mark.parametrize("group", [24, 32])
+def test_pairs_in_more_parts_than_a_warp_has_lanes(group, D, dtype):
+    # a single token's pair over 79 CTAs or more, rows that stay with their lanes (more than 16 a
+    # warp): each lane waits for parts that all lanes read
+    b = Batch([25000], [1], group, 1, D, 16, dtype, seed=30 + group)
+    o, e = b.run()
+    b.check(o, e)
+    for _ in range(20):
+        again = b.run()
+        assert torch.equal(again[0], o) and torch.equal(again[1], e)
+
+
 @pytest.mark.parametrize("R", [95, 96, 97, 1024, 1025, 2300])
 def test_many_requests(R):
     rng = np.random.default_rng(R)

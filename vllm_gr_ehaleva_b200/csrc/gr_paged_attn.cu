@@ -910,7 +910,10 @@ __device__ __forceinline__ bool wait_parts(const Params& P, Shared* sh, int part
     while (ok && ld_acquire(P.flag + (p * 2 + slot) * 4 + warp) != P.token)
       ok = *reinterpret_cast<volatile int*>(&sh->abort) == 0 && gr::global_timer_ns() - since < 10 * gr::kWaitLimitNs;
   }
-  if (__all_sync(0xFFFFFFFFu, ok)) return true;
+  if (__all_sync(0xFFFFFFFFu, ok)) {
+    __syncwarp();   // a vote orders no memory: all lanes read what each lane's flags stand for
+    return true;
+  }
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
 }
