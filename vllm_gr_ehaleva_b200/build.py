@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -70,7 +71,9 @@ def _run(cmd):
 
 def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     """Compiles the sources side by side (those whose object is older than what
-    it is made of; all of them with `force` or extra flags) and links them."""
+    it is made of; all of them with `force` or extra flags) and links them.
+    Objects made with extra flags live in a directory of their own for the time
+    of the call: none is left for another build to take for its own."""
     if not force and not extra_flags and up_to_date():
         return LIB_PATH
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -78,24 +81,26 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     if verbose:
         flags += ["-Xptxas", "-v"]
     flags += list(extra_flags or [])
+    obj_dir = tempfile.mkdtemp(prefix="extra_", dir=OBJ_DIR) if extra_flags else OBJ_DIR
 
     def compile_one(src):
-        obj = os.path.join(OBJ_DIR, src + ".o")
+        obj = os.path.join(obj_dir, src + ".o")
         if not force and not extra_flags and _newer(obj, _inputs(src)):
             return obj, ""
         log = _run([nvcc_path(), *flags, "-c", os.path.join(CSRC, src), "-o", obj + ".tmp.o"])
         os.replace(obj + ".tmp.o", obj)
         return obj, log
 
-    with ThreadPoolExecutor(len(SOURCES)) as pool:
-        done = list(pool.map(compile_one, SOURCES))
-    if verbose:
-        sys.stderr.write("".join(log for _, log in done))
-    _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-o", LIB_PATH + ".tmp", *[obj for obj, _ in done]])
-    os.replace(LIB_PATH + ".tmp", LIB_PATH)
-    if extra_flags:
-        for obj, _ in done:   # objects of another build than the default one are not kept
-            os.remove(obj)
+    try:
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            done = list(pool.map(compile_one, SOURCES))
+        if verbose:
+            sys.stderr.write("".join(log for _, log in done))
+        _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-o", LIB_PATH + ".tmp", *[obj for obj, _ in done]])
+        os.replace(LIB_PATH + ".tmp", LIB_PATH)
+    finally:
+        if extra_flags:
+            shutil.rmtree(obj_dir, ignore_errors=True)
     return LIB_PATH
 
 
