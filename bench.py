@@ -920,7 +920,7 @@ def run_paged(args):
         free = ids[int(have.sum()):].clone()
         k_cache = torch.randn(nb, block, HK, D, device=device, generator=g).to(torch.bfloat16)
         v_cache = torch.randn(nb, block, HK, D, device=device, generator=g).to(torch.bfloat16)
-        k = torch.randn(T, HK, D, device=device, generator=g).to(torch.bfloat16)
+        k, v = (torch.randn(T, HK, D, device=device, generator=g).to(torch.bfloat16) for _ in range(2))
         q = torch.randn(T, H, D, device=device, generator=g).to(torch.bfloat16)
         c, f = i32(cached), i32(fresh)
         beams = dict(beam_tail=i32(np.full(R, tail)), beam_steps=i32(np.full(R, steps))) if steps else {}
@@ -928,7 +928,7 @@ def run_paged(args):
         mx = int(fresh.max())
         iters = min(args.steps, 100)
         ms_t = timed(lambda: extend_block_tables(table, c, f, free, block, T), iters)
-        ms_s = timed(lambda: store_kv(k, k, k_cache, v_cache, m["slot_mapping"]), iters)
+        ms_s = timed(lambda: store_kv(k, v, k_cache, v_cache, m["slot_mapping"]), iters)
         ms_a = timed(lambda: paged_attention(q, k_cache, v_cache, table, m["cu_seqlens_q"], m["seq_lens"], mx, **beams),
                      iters)
         pairs = int((fresh * cached + fresh * (fresh + 1) // 2).sum())
@@ -944,7 +944,8 @@ def run_paged(args):
             "unit": "ms", "higher_is_better": False, "tflops": round(flops / ms_a / 1e9, 1),
             "gbs": round(nbytes / ms_a / 1e6, 1), "block_tables_ms": round(ms_t, 5), "store_ms": round(ms_s, 5),
             "dtype": "bf16", "config": {"requests": R, "tokens": T, "keys": keys, "heads": H, "kv_heads": HK,
-                                        "head_dim": D, "block_size": block, "beam_tail": tail, "beam_steps": steps},
+                                        "head_dim": D, "block_size": block, "beam_tail": tail, "beam_steps": steps,
+                                        "inputs": "the same tensors every call: in L2 where they fit it"},
             "roofline": {"bound": bound, "floor_ms": round(floor_ms, 5), "frac": round(floor_ms / ms_a, 4),
                          "peak_gbs": peak, "peak_tflops": tflops, "peak_kind": peak_kind}}), flush=True)
 
