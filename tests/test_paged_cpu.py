@@ -234,3 +234,30 @@ def test_oracle_block_tables_by_hand():
     assert t.tolist() == [[7, 1, -1], [-1, -1, -1], [9, 8, 2]] and used == 2 and not no_block
     assert cu.tolist() == [0, 3, 3, 4] and lens.tolist() == [6, 0, 9]
     assert slots.tolist() == [31, 4, 5, 8, -1] and pos.tolist() == [3, 4, 5, 8, 0]
+
+
+def _changed_signature(size, stride):
+    return None
+
+
+def _other_answer(size, stride, dtype):
+    return torch.empty(1)
+
+
+@pytest.mark.parametrize("private", [_changed_signature, _other_answer, None])
+def test_allocation_without_torchs_private_entry(monkeypatch, private):
+    # a torch whose entry is gone, takes other arguments or answers otherwise: the public one is taken
+    import importlib.util
+    from vllm_gr_ehaleva_b200.attention import paged
+    if private is None:
+        monkeypatch.delattr(torch._C._dynamo.guards, "_empty_strided_cuda", raising=False)
+    else:
+        monkeypatch.setattr(torch._C._dynamo.guards, "_empty_strided_cuda", private, raising=False)
+    made = []
+    monkeypatch.setattr(torch, "empty_strided", lambda *a, **k: made.append((a, k)) or len(made))
+    spec = importlib.util.spec_from_file_location(paged.__name__, paged.__file__)
+    fresh = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(fresh)
+    for i in (1, 2):
+        assert fresh._empty((2, 3), (3, 1), torch.int32) == i
+    assert made == 2 * [(((2, 3), (3, 1)), dict(dtype=torch.int32, device="cuda"))]
