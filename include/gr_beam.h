@@ -388,7 +388,8 @@ int32_t gr_remux_logprobs(const gr_remux_desc* desc, const int32_t* row_w, const
  * bits, and tokens beyond num_tokens give GR_DEVERR_BAD_RECORD: such a length
  * pair counts as no new token (a negative cached as 0), such tokens have no
  * entry.  err may be NULL; bits are OR-ed into it.  positions may be NULL.
- * num_seqs at most 2^31 - 4096 (GR_ERR_BAD_DESC).
+ * Outputs must not overlap inputs or one another (block_table alone is updated
+ * in place).  num_seqs at most 2^31 - 4096 (GR_ERR_BAD_DESC).
  * The reference leaves this to vLLM's host code (v1/worker/block_table.py,
  * NumPy loops and copies per step); its builder consumes the result
  * (beam_attn.py:432-476). */
@@ -415,9 +416,10 @@ int32_t gr_extend_block_tables(const gr_block_table_desc* desc, int32_t* block_t
  * and the same for V.  Slots < 0 are skipped (padding); slots outside
  * [0, num_blocks * block_size) are skipped and set GR_DEVERR_BAD_SLOT in *err
  * (err may be NULL).  The slots of one call must differ from one another: of two
- * rows for one slot an unspecified mix may remain.  Strides are in elements.
+ * rows for one slot an unspecified mix may remain.  k and v must not lie in the
+ * caches.  Strides are in elements.
  * num_heads * head_dim at most 2^31 - 1024 (GR_ERR_BAD_DESC).
- * Replaces vLLM's reshape_and_cache_flash as the reference calls it
+ * Replaces the cache write that the reference's backend calls
  * (beam_attn.py:727-732). */
 typedef struct gr_kv_store_desc {
   int64_t num_tokens;
@@ -447,9 +449,13 @@ int32_t gr_store_kv(const gr_kv_store_desc* desc, const void* k, const void* v, 
  * its beam.  beam_tail / beam_steps may both be NULL.  Query head h reads KV
  * head h / (num_heads / num_kv_heads).  With s_k = scale * q.k over the seen keys
  *     lse = ln sum_k exp(s_k)          out = sum_k exp(s_k - lse) v_k
- * out has q's type, lse is fp32 [num_tokens][num_heads] (may be NULL).  A token
- * that sees no key gets out = 0 and lse = -inf.  Rows of tokens that belong to
- * no request are left as they were.
+ * out has q's type, lse is fp32 [num_tokens][num_heads] (may be NULL).  Scores,
+ * sums and accumulators are fp32; the weights exp(s_k - .) are rounded once to
+ * q's type before they multiply v_k (each off by at most half a step: 2^-8 bf16,
+ * 2^-11 f16, relative), the sum takes them unrounded, and out is rounded once.
+ * A token that sees no key gets out = 0 and lse = -inf.  Rows of tokens that
+ * belong to no request are left as they were.  out and lse must not overlap the
+ * inputs.
  * Cache rows at positions >= L_r are never used, whatever they hold.  Rows at
  * positions < L_r that a token does not see still enter as 0 * v: V has to be
  * finite there.
@@ -501,9 +507,14 @@ typedef struct gr_paged_attn_io {
 } gr_paged_attn_io;
 
 /* Bytes of workspace gr_paged_attention() needs for `desc` (256-byte aligned,
- * contents need not be initialised; calls that share it must not overlap).  A
- * captured call that has set GR_DEVERR_TIMEOUT must be captured anew before it
- * is replayed: the workspace may hold parts of the run that gave up. */
+ * contents need not be initialised; calls that share it must not overlap): 10 to
+ * 42 MB by head_dim and kernel, two partial tiles for each CTA whether or not the
+ * call cuts a pair, besides the plan.
+ * Every wait of the kernel is bounded: about 2 s for a copy or a product, 32 s
+ * for what lasts as long as a (query block, KV head) pair, 20 s for another CTA's
+ * part.  One that runs out sets GR_DEVERR_TIMEOUT and outputs stay incomplete;
+ * with err NULL nothing tells.  A captured call that has set it must be captured
+ * anew before it is replayed: the workspace may hold parts of the run that gave up. */
 int32_t gr_paged_attention_workspace_size(const gr_paged_attn_desc* desc, size_t* bytes);
 
 int32_t gr_paged_attention(const gr_paged_attn_desc* desc, const gr_paged_attn_io* io, void* workspace,

@@ -216,9 +216,11 @@ def store_kv(k, v, k_cache, v_cache, slot_mapping, *, err=None) -> None:
     """Writes the rows k[t], v[t] ([T, num_kv_heads, head_dim]) into the cache slots
     slot_mapping[t] (int64 [T], or int32, which is widened; slot = block * block_size +
     offset).  Slots < 0 are skipped; slots behind the cache are skipped and set
-    GR_DEVERR_BAD_SLOT in `err`.  The slots of one call must differ.  Any strides; 1-, 2- and
-    4-byte elements; rows are copied as they are, so k and the cache have one dtype.  The
-    inverse of extract_suffix_kv."""
+    GR_DEVERR_BAD_SLOT in `err`.  The slots of one call must differ, and k and v must not lie in
+    the caches.  Any strides (rows of whole 16-byte vectors in the row and in the cache are
+    copied as such, others by the element, some four times slower); 1-, 2- and 4-byte elements; rows
+    are copied as they are, so k and the cache have one dtype.  The inverse of
+    extract_suffix_kv."""
     if slot_mapping.dtype == _I32:
         slot_mapping = slot_mapping.to(_I64)
     key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, k_cache.shape, k_cache.stride(),
@@ -300,14 +302,22 @@ def paged_attention(q, k_cache, v_cache, block_table, cu_seqlens_q, seq_lens, ma
     Returns out ([T, num_heads, head_dim], q's dtype; pass `out` to write into a tensor of
     yours), with return_lse also the fp32 [T, num_heads] natural log-sum-exp of the scaled
     scores.  A token without keys gets 0 and -inf; rows of tokens that belong to no request
-    are left as they were (unspecified in a new `out`).  scale defaults to head_dim ** -0.5.
+    are left as they were (unspecified in a new `out`).  `out` must not overlap the inputs;
+    gradients are not computed.  scale defaults to head_dim ** -0.5.
     V has to be finite at positions below seq_lens; what blocks hold behind does not matter.
+
+    Scores, sums and accumulators are fp32.  The softmax's weights are rounded once to q's
+    dtype before they multiply V (each off by at most half a step: 2^-8 in bf16, 2^-11 in f16,
+    relative; their sum takes them unrounded), and out is rounded once.
 
     head_dim: a multiple of 8 up to 256; block_size: a multiple of 8; num_heads /
     num_kv_heads up to 128; unit stride in head_dim, other strides multiples of 8 elements,
     16-byte aligned tensors.  Block ids outside the cache read as zero rows and set
     GR_DEVERR_BAD_SLOT in `err` (optional int32 device tensor); lengths outside the table's
-    row or the tokens are clamped and set GR_DEVERR_BAD_RECORD."""
+    row or the tokens are clamped and set GR_DEVERR_BAD_RECORD.  A wait inside the kernel that
+    runs out (2 to 32 seconds, by what it waits for) sets GR_DEVERR_TIMEOUT and leaves the
+    outputs incomplete, of which nothing tells without `err`; a captured call that has set it
+    must be captured anew."""
     # a longer bound than any query tile picks the same kernel
     max_seqlen_q, causal = min(int(max_seqlen_q), 129), bool(causal)
     scale = None if scale is None else float(scale)

@@ -37,13 +37,17 @@
 // tensor pipe; one tile (kNQ = 1: no query of more than 128 rows, or heads above
 // 128, whose accumulators leave no room) alternates two score buffers instead and
 // has four more loading warps.  Heads above 128 move their tiles as two halves of
-// 128 columns.  Every wait is bounded (GR_DEVERR_TIMEOUT).
+// 128 columns.  The kernel is picked for the whole batch by its longest query: one
+// chunk beside 64 single tokens puts them into the kernel with two tiles (263 us
+// instead of 183).  Every wait is bounded (GR_DEVERR_TIMEOUT).
 //
 // Bound and measured (32 query heads over 8 KV heads of 128, blocks of 16): 64
-// single tokens over 2.5 GB of cache 6.3 TB/s, HBM, 96 % of a plain copy's rate; a
-// prompt of 8192 1080 to 1170 TFLOP/s, the chain scores - softmax - product of a
-// query tile (exponential unit and tensor pipe each near half of their rate), and
-// in long runs the power limit.
+// single tokens over 2.5 GB of cache 6.4 TB/s, HBM, 98 % of a plain copy's rate
+// (over 1.1 GB 6.0 TB/s for some milliseconds, 5.0 in runs of seconds, where the
+// power limit holds); a prompt of 8192 1060 TFLOP/s for some milliseconds and 920 to
+// 1000 in longer runs: the chain scores - softmax - product of a query tile
+// (exponential unit and tensor pipe each near half of their rate), then the power
+// limit (1.4 to 1.7 GHz).
 
 #include <atomic>
 #include <chrono>
@@ -154,7 +158,7 @@ struct Params {
   uint32_t div_mul, div_shift;     // x / block_size = (x * div_mul >> 32) >> div_shift for x < 2^31
   int out32;                       // output rows start on 32 bytes
   int flags;                       // 1: copies are not issued (test hook)
-  float scale_log2, scale;
+  float scale_log2;
   // plan and partials in the workspace
   int64_t* pre;                    // [items + 1] units of one KV head before each query block
   int2* item;                      // request, block
@@ -1591,7 +1595,6 @@ extern "C" int32_t gr_paged_attention(const gr_paged_attn_desc* d, const gr_page
             (d->out_stride_tok % 16 == 0 || d->num_tokens == 1) && (d->out_stride_head % 16 == 0 || d->num_heads == 1);
   const char* stall = std::getenv("GR_TEST_STALL_COPIES");
   P.flags = stall && stall[0] == '1' ? 1 : 0;
-  P.scale = d->scale;
   P.scale_log2 = d->scale * gr::kLog2e;
   P.run = reinterpret_cast<Run*>(ws + l.run);
   P.flag = reinterpret_cast<uint64_t*>(ws + l.flag);
