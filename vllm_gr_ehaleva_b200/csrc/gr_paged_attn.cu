@@ -698,6 +698,12 @@ __device__ __forceinline__ void load_role(const Params& P, Shared* sh, uint32_t 
     }
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0 && P.err) atomicOr(P.err, GR_DEVERR_BAD_SLOT);
+  // stays until the products have used the run's last tile, whichever warps loaded it: a role that
+  // gives up after this warp's last issue finds it here, to wait for what is still in flight
+  {
+    const bool lap = ring.stage == 0;
+    wait(sh, &sh->empty[lap ? S::kStages - 1 : ring.stage - 1], ring.phase ^ static_cast<uint32_t>(lap));
+  }
   if (aborted(sh)) {
     // gave up: wait (bounded) for this warp's copies in flight before the shared memory goes
     for (int i = 0; i < S::kStages; ++i) {
